@@ -6,4 +6,4 @@ these modules mirror the reference's Go packages on the host side.
 """
 from . import capi  # noqa: F401
 
-__all__ = ["capi", "runtime", "dft", "mel", "agabor", "sound", "batch", "synth"]
+__all__ = ["capi", "runtime", "dft", "mel", "agabor", "sound", "batch", "synth", "kwta", "norm", "scan"]

@@ -11,6 +11,8 @@ LIB_PATH = os.path.join(HERE, "libauditory_hip.so")
 
 AUD_OK, AUD_EINVAL, AUD_EHIP, AUD_ERCCL, AUD_ENOMEM, AUD_ESHORT, AUD_EBROKEN = 0, 1, 2, 3, 4, 5, 6
 AUD_RESIDENT_AUTO_BYTES = 8 << 20   # include/auditory_hip.h
+AUD_BF16, AUD_F16 = 3, 4              # activations of the feature-map and frame-sequence operators
+AUD_ACT_NONE, AUD_ACT_RELU, AUD_ACT_SILU, AUD_ACT_GELU = 0, 1, 2, 3
 AUD_F64, AUD_F32, AUD_I16 = 0, 1, 2   # AUD_F64 == 0: a zeroed PlanDesc is the float64 (conforming) plan
 AUD_FAST_F32 = AUD_F32                # compute_dtype opt-in: the float32 kernels (never a default)
 
@@ -72,6 +74,21 @@ class KwtaParams(C.Structure):
     _fields_ = [("on", C.c_int32), ("iters", C.c_int32), ("del_act_thr", C.c_float),
                 ("lay_fffb", FffbParams), ("pool_fffb", FffbParams), ("xx1", Nxx1Params),
                 ("act_tau", C.c_float), ("gbar", C.c_float * 4), ("erev", C.c_float * 4)]
+
+
+class NormParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "act", "n_items", "rows", "channels", "groups")] + \
+        [("eps", C.c_float), ("reserved", C.c_int32)] + [(n, C.c_int64) for n in ("x_item", "x_row", "dy_item", "dy_row")]
+
+
+class ConvParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "act", "n_items", "steps", "channels", "taps")] + \
+        [(n, C.c_int64) for n in ("x_item", "x_row", "dy_item", "dy_row")]
+
+
+class ScanParams(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("dtype", "softplus", "n_items", "steps", "channels", "groups", "states", "reserved")] + \
+        [(n + k, C.c_int64) for n in ("u", "delta", "z", "b", "c", "dy") for k in ("_item", "_row")]
 
 
 # every symbol include/auditory_hip.h declares: name -> (restype, argtypes)
@@ -143,6 +160,16 @@ SYMBOLS = {
     "aud_kwta_defaults": (None, [C.POINTER(KwtaParams)]),
     "aud_kwta_batch_dev": (C.c_int, [_VP, C.POINTER(KwtaParams), _VP, _VP] + [C.c_int] * 7 + [_VP, C.c_int, _VP, _VP]),
     "aud_kwta_batch_host": (C.c_int, [_VP, C.POINTER(KwtaParams), _VP, _VP] + [C.c_int] * 7 + [_VP, C.c_int, _VP]),
+    "aud_group_norm_workspace_bytes": (C.c_int, [C.POINTER(NormParams), C.c_int, C.POINTER(C.c_int64)]),
+    "aud_group_norm_batch_dev": (C.c_int, [_VP, C.POINTER(NormParams)] + [_VP] * 7 + [C.c_int64, _VP]),
+    "aud_group_norm_grad_dev": (C.c_int, [_VP, C.POINTER(NormParams)] + [_VP] * 10 + [C.c_int64, _VP]),
+    "aud_causal_conv_batch_dev": (C.c_int, [_VP, C.POINTER(ConvParams)] + [_VP] * 8),
+    "aud_causal_conv_workspace_bytes": (C.c_int, [C.POINTER(ConvParams), C.POINTER(C.c_int64)]),
+    "aud_causal_conv_grad_dev": (C.c_int, [_VP, C.POINTER(ConvParams)] + [_VP] * 12 + [C.c_int64, _VP]),
+    "aud_scan_workspace_bytes": (C.c_int, [C.POINTER(ScanParams), C.c_int, C.POINTER(C.c_int64)]),
+    "aud_scan_kept_floats": (C.c_int, [C.POINTER(ScanParams), C.POINTER(C.c_int64)]),
+    "aud_scan_batch_dev": (C.c_int, [_VP, C.POINTER(ScanParams)] + [_VP] * 14 + [C.c_int64, _VP]),
+    "aud_scan_grad_dev": (C.c_int, [_VP, C.POINTER(ScanParams)] + [_VP] * 22 + [C.c_int64, _VP]),
     "aud_comm_unique_id": (C.c_int, [_VP]),
     "aud_comm_init": (C.c_int, [_VP, C.c_int, C.c_int, _VP]),
     "aud_comm_destroy": (C.c_int, [_VP]),

@@ -46,6 +46,8 @@ extern "C" {
 #define AUD_F64 0
 #define AUD_F32 1
 #define AUD_I16 2 /* raw 16-bit PCM; normalised on device by /0x7FFF (sound.go:138) */
+#define AUD_BF16 3 /* bfloat16 / IEEE half: activations of the feature-map and frame-sequence operators only */
+#define AUD_F16 4
 #define AUD_FAST_F32 AUD_F32 /* aud_plan_desc.compute_dtype: the non-conforming fast plan, never a default */
 
 typedef struct aud_ctx aud_ctx;
@@ -478,6 +480,95 @@ int aud_kwta_batch_dev(aud_ctx* ctx, const aud_kwta_params* k, const float* raw,
 int aud_kwta_batch_host(aud_ctx* ctx, const aud_kwta_params* k, const float* raw, float* act, int n_items, int d0,
                         int d1, int d2, int d3, int pool_level, int start_from_raw, float* pool_state,
                         int sum_order, int32_t* cycles);
+
+/* ---- feature-map and frame-sequence operators ----------------------------------------------
+ * What a network puts right behind the tensors above, for values and for gradients: group norm with an activation on a
+ * channels-last map (beside the k-WTA stage: map -> activation), a short causal convolution over frames and a selective state
+ * space scan over frames (beside dft.PrevSmooth and the MFCC deltas: a learned recurrence and a learned filter in place of
+ * the fixed ones), for whole utterances and for one frame at a time with the state carried between calls.
+ *
+ * Common rules
+ *  - dtype AUD_F32, AUD_BF16 or AUD_F16 is the type of the activations (x, y, dy, dx, u, delta, z, B, C, conv states);
+ *    parameters, their gradients, statistics and scan states are float32, and so is every sum.
+ *  - *_item / *_row are the distances, in elements, between items and between rows (positions, frames) of an input; the
+ *    channels of a row are contiguous.  Outputs are contiguous.  Inputs of any alignment that their type allows are taken;
+ *    16-byte aligned pointers and strides run faster.
+ *  - lengths: int32 [n_items] in device memory, or NULL (every item is full).  Rows at and behind an item's length are
+ *    padding: whatever they hold (NaN too) has no effect; outputs and gradients are written as zero there.  A value outside
+ *    [0, rows] counts as the nearer end.
+ *  - Results do not depend on other items of the batch, sums have a fixed order (no atomics): the same call gives the same bits.
+ *  - An output must not overlap an input, except state_out, which may be the state itself (same pointer).
+ *  - workspace: device memory, 16-byte aligned, of the size that the _workspace_bytes function says for the SAME parameters;
+ *    contents undefined before and after; NULL where that size is 0.  Calls on different streams, and captured graphs that may
+ *    run side by side, need workspaces of their own.  All calls only enqueue kernels and can be captured.
+ *  - Parameter structs hold no pointers. */
+#define AUD_ACT_NONE 0
+#define AUD_ACT_RELU 1
+#define AUD_ACT_SILU 2 /* p / (1 + e^-p) */
+#define AUD_ACT_GELU 3 /* p (1 + erf(p / sqrt 2)) / 2; group norm only */
+
+/* group norm: x [n_items, rows, channels], `groups` groups of neighbouring channels, each normalised over rows x its channels
+ * (the biased variance), then weight, bias and the activation.  1 <= channels <= 4096, a multiple of groups; eps > 0. */
+typedef struct {
+    int32_t dtype, act, n_items, rows, channels, groups;
+    float eps;
+    int32_t reserved; /* 0 */
+    int64_t x_item, x_row;
+    int64_t dy_item, dy_row; /* gradients only */
+} aud_norm_params;
+int aud_group_norm_workspace_bytes(const aud_norm_params* p, int gradients, int64_t* bytes);
+/* weight, bias float32 [channels] or NULL (1, 0); y [n_items, rows, channels]; stats float32 [n_items, groups, 2] = (mean,
+ * 1 / sqrt(variance + eps)), what the gradients need, or NULL */
+int aud_group_norm_batch_dev(aud_ctx* ctx, const aud_norm_params* p, const void* x, const float* weight, const float* bias,
+                             const int32_t* lengths, void* y, float* stats, void* workspace, int64_t workspace_bytes, void* stream);
+/* dx as y; dweight, dbias float32 [channels] (sums over the batch) or NULL */
+int aud_group_norm_grad_dev(aud_ctx* ctx, const aud_norm_params* p, const void* dy, const void* x, const float* stats,
+                            const float* weight, const float* bias, const int32_t* lengths, void* dx, float* dweight,
+                            float* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* causal convolution: x [n_items, steps, channels], weight float32 [channels, taps] (the last tap meets the current frame),
+ * 1 <= taps <= 4; act AUD_ACT_NONE or AUD_ACT_SILU.  state [n_items, taps - 1, channels], oldest first: the inputs in front of
+ * x (NULL: zeros); state_out: the last taps - 1 inputs of each item, counted to its length -- the next call's state. */
+typedef struct {
+    int32_t dtype, act, n_items, steps, channels, taps;
+    int64_t x_item, x_row;
+    int64_t dy_item, dy_row; /* gradients only */
+} aud_conv_params;
+int aud_causal_conv_batch_dev(aud_ctx* ctx, const aud_conv_params* p, const void* x, const float* weight, const float* bias,
+                              const void* state, const int32_t* lengths, void* y, void* state_out, void* stream);
+int aud_causal_conv_workspace_bytes(const aud_conv_params* p, int64_t* bytes); /* of the gradients */
+/* dstate_out: gradient of state_out, or NULL; dstate [n_items, taps - 1, channels], dweight, dbias: or NULL */
+int aud_causal_conv_grad_dev(aud_ctx* ctx, const aud_conv_params* p, const void* dy, const void* x, const float* weight,
+                             const float* bias, const void* state, const int32_t* lengths, const void* dstate_out, void* dx,
+                             float* dweight, float* dbias, void* dstate, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* selective scan: u, delta, z [n_items, steps, channels], B, C [n_items, steps, groups, states] (groups and states
+ * contiguous; a group's B and C serve channels / groups neighbouring channels), A float32 [channels, states], D and
+ * delta_bias float32 [channels] or NULL, z NULL for no gate.  1 <= states <= 64; channels a multiple of groups.
+ *   dt = softplus(delta + delta_bias) (softplus = 0: without it);  h = exp(dt A) h + dt u B;  y = (sum h C + D u) silu(z)
+ * state, state_out float32 [n_items, channels, states]: the state in front of the first frame (NULL: zeros) and behind the
+ * last of each item.  steps = 1 is the streaming form: one launch, no workspace. */
+typedef struct {
+    int32_t dtype, softplus, n_items, steps, channels, groups, states;
+    int32_t reserved; /* 0 */
+    int64_t u_item, u_row, delta_item, delta_row, z_item, z_row, b_item, b_row, c_item, c_row;
+    int64_t dy_item, dy_row; /* gradients only */
+} aud_scan_params;
+int aud_scan_workspace_bytes(const aud_scan_params* p, int gradients, int64_t* bytes);
+/* floats of the `kept` table: the states that aud_scan_grad_dev starts from, one set for every 16 frames */
+int aud_scan_kept_floats(const aud_scan_params* p, int64_t* floats);
+int aud_scan_batch_dev(aud_ctx* ctx, const aud_scan_params* p, const void* u, const void* delta, const float* A, const void* B,
+                       const void* C, const float* D, const void* z, const float* delta_bias, const float* state,
+                       const int32_t* lengths, void* y, float* state_out, float* kept, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+/* kept: as aud_scan_batch_dev wrote it for the same inputs.  dstate_out: gradient of state_out, or NULL.  du, ddelta (and dz
+ * where z is given) [n_items, steps, channels]; dB, dC [n_items, steps, groups, states]; dA float32 [channels, states]; dD,
+ * ddelta_bias float32 [channels], dstate float32 [n_items, channels, states]: or NULL. */
+int aud_scan_grad_dev(aud_ctx* ctx, const aud_scan_params* p, const void* dy, const void* u, const void* delta, const float* A,
+                      const void* B, const void* C, const float* D, const void* z, const float* delta_bias,
+                      const int32_t* lengths, const float* kept, const float* dstate_out, void* du, void* ddelta, float* dA,
+                      void* dB, void* dC, float* dD, void* dz, float* ddelta_bias, float* dstate, void* workspace,
+                      int64_t workspace_bytes, void* stream);
 
 /* ---- multi-GPU reassembly (one process per GPU, RCCL over xGMI) ------------------ */
 

@@ -53,6 +53,27 @@ inline void __builtin_amdgcn_sched_barrier(int) {}
 inline float absmax3(float m, float x, float y) { return fmaxf(m, fmaxf(fabsf(x), fabsf(y))); }
 inline float __builtin_amdgcn_logf(float v) { return log2f(v); }  // v_log_f32 is a base-2 logarithm
 inline double __builtin_amdgcn_rcp(double v) { return double(float(1.0 / v)); }  // v_rcp_f64: an APPROXIMATION (~2^-26), refined by the caller
+inline float __builtin_amdgcn_exp2f(float v) { return exp2f(v); }
+inline float __builtin_amdgcn_rcpf(float v) { return 1.0f / v; }
+namespace aud_emul {
+// IEEE half <-> float, round to nearest even (g++ has no half type here)
+inline float half_to_float(uint16_t h) {
+    const int e = (h >> 10) & 31, m = h & 1023;
+    const float v = e == 31 ? (m ? NAN : INFINITY) : e ? std::ldexp(float(1024 + m), e - 25) : std::ldexp(float(m), -24);
+    return h & 0x8000 ? -v : v;
+}
+inline uint16_t float_to_half(float f) {
+    const uint16_t s = std::signbit(f) ? 0x8000 : 0;
+    if (std::isnan(f)) return uint16_t(s | 0x7E00);
+    const float a = std::fabs(f);
+    if (a >= 65520.f) return uint16_t(s | 0x7C00);
+    if (a < 6.103515625e-05f) return uint16_t(s | uint16_t(std::nearbyint(std::ldexp(a, 24))));  // (1024 steps: the smallest normal)
+    int e;
+    std::frexp(a, &e);
+    const int m = int(std::nearbyint(std::ldexp(a, 11 - e)));  // 1024 .. 2048
+    return uint16_t(s | ((e + 14) * 1024 + (m - 1024)));
+}
+}  // namespace aud_emul
 // same-value races the 20 x 10 wave kernel has by design (shadow lanes): ThreadSanitizer is told to look away
 #if defined(__SANITIZE_THREAD__)
 extern "C" void AnnotateIgnoreWritesBegin(const char*, int);
