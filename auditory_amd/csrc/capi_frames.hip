@@ -8,6 +8,7 @@ using namespace audc;
 namespace {
 
 constexpr int64_t kMaxElements = int64_t(1) << 40;
+constexpr int32_t kMaxRows = 1 << 30;  // rows of an item: a tile behind them still counts in 32 bits
 constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
 
 // the context's device for the length of a call; the caller's current device is put back
@@ -76,7 +77,7 @@ const char* norm_bad(const aud_norm_params* p, bool grad) {
     if (!p) return "null parameters";
     if (!known_type(p->dtype)) return "dtype must be AUD_F32, AUD_BF16 or AUD_F16";
     if (p->act < AUD_ACT_NONE || p->act > AUD_ACT_GELU) return "unknown activation";
-    if (p->n_items < 0 || p->rows < 0 || p->channels < 1 || p->groups < 1) return "bad shape";
+    if (p->n_items < 0 || p->rows < 0 || p->rows > kMaxRows || p->channels < 1 || p->groups < 1) return "bad shape";
     if (p->channels > 4096) return "group norm takes at most 4096 channels";
     if (p->channels % p->groups) return "channels must be a multiple of groups";
     if (!(p->eps > 0.f)) return "eps must be positive";
@@ -87,8 +88,8 @@ const char* norm_bad(const aud_norm_params* p, bool grad) {
     return nullptr;
 }
 // (the route goes by sizes alone, so that the workspace has one size whatever the alignment)
-aud::NormRoute norm_route_of(const aud_norm_params* p, bool aligned, bool grad) {
-    return aud::norm_route(p->dtype, p->n_items > 0 ? p->n_items : 1, p->rows, p->channels, aligned, grad);
+aud::NormRoute norm_route_of(const aud_norm_params* p, int align, bool grad) {
+    return aud::norm_route(p->dtype, p->n_items > 0 ? p->n_items : 1, p->rows, p->channels, p->groups, align, grad);
 }
 
 // ---- causal convolution ----
@@ -96,7 +97,7 @@ const char* conv_bad(const aud_conv_params* p, bool grad) {
     if (!p) return "null parameters";
     if (!known_type(p->dtype)) return "dtype must be AUD_F32, AUD_BF16 or AUD_F16";
     if (p->act != AUD_ACT_NONE && p->act != AUD_ACT_SILU) return "the convolution's activation is AUD_ACT_NONE or AUD_ACT_SILU";
-    if (p->n_items < 0 || p->steps < 0 || p->channels < 1) return "bad shape";
+    if (p->n_items < 0 || p->steps < 0 || p->steps > kMaxRows || p->channels < 1) return "bad shape";
     if (p->taps < 1 || p->taps > 4) return "taps must be 1 to 4";
     if (int64_t(p->n_items) * p->steps > kMaxElements / p->channels) return "tensor too large";
     const Input x{nullptr, p->n_items, p->steps, p->channels, p->x_item, p->x_row};
@@ -110,7 +111,7 @@ int64_t conv_tiles(const aud_conv_params* p, int T) { return p->steps > 0 ? (int
 const char* scan_bad(const aud_scan_params* p, bool gated, bool grad) {
     if (!p) return "null parameters";
     if (!known_type(p->dtype)) return "dtype must be AUD_F32, AUD_BF16 or AUD_F16";
-    if (p->n_items < 0 || p->steps < 0 || p->channels < 1 || p->groups < 1) return "bad shape";
+    if (p->n_items < 0 || p->steps < 0 || p->steps > kMaxRows || p->channels < 1 || p->groups < 1) return "bad shape";
     if (p->channels % p->groups) return "channels must be a multiple of groups";
     if (p->states < 1 || p->states > 64) return "states must be 1 to 64";
     if (int64_t(p->n_items) * (p->steps > 0 ? p->steps : 1) > kMaxElements / (int64_t(p->channels) * p->states)) return "tensor too large";
@@ -123,18 +124,26 @@ const char* scan_bad(const aud_scan_params* p, bool gated, bool grad) {
     if ((gated && !z.strides_ok()) || (grad && !d.strides_ok())) return "strides make rows or items overlap";
     return nullptr;
 }
-aud::ScanRoute scan_route_of(const aud_scan_params* p) {
-    return aud::scan_route(p->n_items > 0 ? p->n_items : 1, p->steps, p->channels, p->groups, p->states);
+aud::ScanRoute scan_route_of(const aud_scan_params* p, bool grad) {
+    return aud::scan_route(p->n_items > 0 ? p->n_items : 1, p->steps, p->channels, p->groups, p->states, grad);
 }
 int64_t scan_tiles(const aud_scan_params* p) { return (int64_t(p->steps) + aud::kScanTile - 1) / aud::kScanTile; }
-struct ScanSpace {  // floats of the gradients' workspace: chunk sums | dB and dC by block | parameter sums by chunk
-    int64_t sums, bc, part;
-};
 int64_t up4(int64_t n) { return (n + 3) & ~int64_t(3); }
-ScanSpace scan_space(const aud_scan_params* p, const aud::ScanRoute& r) {
-    return {up4(aud::scan_sums_floats(r, p->n_items, p->channels, p->states)),
-            up4(2 * int64_t(r.blocks) * p->n_items * p->steps * p->groups * p->states),
-            int64_t(p->n_items) * r.chunks * (p->states + 2) * p->channels};
+struct ScanSpace {  // floats of the workspace: B and C as a table | chunk sums | gradients: dB and dC by block, parameter sums by chunk
+    int64_t table, sums, bc, part;
+    int64_t all() const { return table + sums + bc + part; }
+};
+ScanSpace scan_space(const aud_scan_params* p, const aud::ScanRoute& r, bool grad) {
+    const int64_t rows = int64_t(p->n_items) * p->groups;
+    ScanSpace s{rows * scan_tiles(p) * aud::kScanTile * 2 * aud::scan_padded_states(p->states),
+                up4(aud::scan_sums_floats(r, p->n_items, p->channels, p->states)), 0, 0};
+    if (grad) {
+        s.bc = r.blocks > 1 ? up4(2 * int64_t(r.blocks) * rows * p->steps * p->states) : 0;
+        s.part = int64_t(p->n_items) * r.chunks * (p->states + 2) * p->channels;
+    } else if (p->steps == 1) {
+        s.table = 0;  // (the one-frame kernel)
+    }
+    return s;
 }
 void fill_scan(const aud_scan_params* p, const aud::ScanRoute& r, aud::ScanArgs* a) {
     a->B = p->n_items;
@@ -155,8 +164,8 @@ extern "C" {
 
 int aud_group_norm_workspace_bytes(const aud_norm_params* p, int gradients, int64_t* bytes) {
     if (!bytes || norm_bad(p, gradients != 0)) return AUD_EINVAL;
-    const aud::NormRoute r = norm_route_of(p, true, gradients != 0);
-    *bytes = 4 * aud::norm_workspace_floats(r, p->n_items, p->channels, p->groups, gradients != 0, false);
+    const aud::NormRoute r = norm_route_of(p, 16, gradients != 0);
+    *bytes = 4 * aud::norm_workspace_floats(r, p->n_items, p->channels, p->groups, gradients != 0);
     return AUD_OK;
 }
 
@@ -178,15 +187,15 @@ int aud_group_norm_batch_dev(aud_ctx* c, const aud_norm_params* p, const void* x
     const Range outs[] = {{y, n * e}, {stats, st}, {workspace, need}};
     const Range ins[] = {{x, in.span(e)}, {weight, ch}, {bias, ch}, {lengths, 4 * int64_t(p->n_items)}};
     if (clash(outs, 3, ins, 4)) return fail(c, AUD_EINVAL, "an output overlaps another buffer");
-    const bool aligned = in.aligned(16, e) && at(y, 16);
-    const aud::NormRoute r = norm_route_of(p, aligned, false);
-    if (int64_t(p->n_items) * r.chunks > kMaxGrid) return fail(c, AUD_EINVAL, "too many items");
+    const int align = in.aligned(16, e) && at(y, 16) ? 16 : in.aligned(8, e) && at(y, 8) ? 8 : e;
+    const aud::NormRoute r = norm_route_of(p, align, false);
+    if (int64_t(p->n_items) * r.chunks > kMaxGrid - 64 || int64_t(p->n_items) * (p->channels / 32 + 1) > kMaxGrid) return fail(c, AUD_EINVAL, "too many items");
     const OnDevice device(c);
     AUD_HIP(c, device.err);
     aud::NormArgs a{};
     a.x = x, a.weight = weight, a.bias = bias, a.lengths = lengths, a.out = y;
     a.part = static_cast<float*>(workspace);
-    a.stats = stats ? stats : a.part + (need / 4 - 2 * int64_t(p->n_items) * p->groups);
+    a.stats = stats || !r.join ? stats : a.part + (need / 4 - 2 * int64_t(p->n_items) * p->groups);
     a.B = p->n_items, a.S = p->rows, a.C = p->channels, a.G = p->groups;
     a.xi = p->x_item, a.xr = p->x_row, a.eps = p->eps;
     a.chunks = r.chunks, a.chunk_rows = r.chunk_rows;
@@ -221,9 +230,9 @@ int aud_group_norm_grad_dev(aud_ctx* c, const aud_norm_params* p, const void* dy
             AUD_HIP(c, aud::launch_column_sums(nullptr, 0, p->channels, 0, 2, nullptr, dweight, dbias, static_cast<hipStream_t>(stream)));
         return AUD_OK;
     }
-    const bool aligned = in.aligned(16, e) && g.aligned(16, e) && at(dx, 16);
-    const aud::NormRoute r = norm_route_of(p, aligned, true);
-    if (int64_t(p->n_items) * r.chunks > kMaxGrid) return fail(c, AUD_EINVAL, "too many items");
+    const int align = in.aligned(16, e) && g.aligned(16, e) && at(dx, 16) ? 16 : in.aligned(8, e) && g.aligned(8, e) && at(dx, 8) ? 8 : e;
+    const aud::NormRoute r = norm_route_of(p, align, true);
+    if (int64_t(p->n_items) * r.chunks > kMaxGrid - 64 || int64_t(p->n_items) * (p->channels / 32 + 1) > kMaxGrid) return fail(c, AUD_EINVAL, "too many items");
     aud::NormArgs a{};
     a.x = x, a.dy = dy, a.weight = weight, a.bias = bias, a.lengths = lengths, a.out = dx;
     a.stats = const_cast<float*>(stats);  // (only read)
@@ -315,9 +324,7 @@ int aud_causal_conv_grad_dev(aud_ctx* c, const aud_conv_params* p, const void* d
 
 int aud_scan_workspace_bytes(const aud_scan_params* p, int gradients, int64_t* bytes) {
     if (!bytes || scan_bad(p, false, false)) return AUD_EINVAL;
-    const aud::ScanRoute r = scan_route_of(p);
-    const ScanSpace s = scan_space(p, r);
-    *bytes = 4 * (gradients ? s.sums + s.bc + s.part : s.sums);
+    *bytes = 4 * scan_space(p, scan_route_of(p, gradients != 0), gradients != 0).all();
     return AUD_OK;
 }
 
@@ -344,7 +351,7 @@ int aud_scan_batch_dev(aud_ctx* c, const aud_scan_params* p, const void* u, cons
         if (!i.aligned(e, e)) return fail(c, AUD_EINVAL, "pointer not aligned to its type");
     if (!at(y, e) || !at(A, 4) || !at(D, 4) || !at(delta_bias, 4) || !at(state, 4) || !at(state_out, 4) || !at(kept, 4) || !at(lengths, 4))
         return fail(c, AUD_EINVAL, "pointer not aligned to its type");
-    const aud::ScanRoute r = scan_route_of(p);
+    const aud::ScanRoute r = scan_route_of(p, false);
     int64_t need = 0, kf = 0;
     (void)aud_scan_workspace_bytes(p, 0, &need);
     (void)aud_scan_kept_floats(p, &kf);
@@ -354,14 +361,15 @@ int aud_scan_batch_dev(aud_ctx* c, const aud_scan_params* p, const void* u, cons
     const Range ins[] = {{u, in[0].span(e)}, {delta, in[1].span(e)}, {z, z ? in[2].span(e) : 0}, {B, in[3].span(e)}, {C, in[4].span(e)},
                          {A, ch * p->states}, {D, ch}, {delta_bias, ch}, {lengths, 4 * ni}, {state == state_out ? nullptr : state, 4 * ns}};
     if (clash(outs, 4, ins, 10)) return fail(c, AUD_EINVAL, "an output overlaps another buffer");
-    if (ni * r.chunks > kMaxGrid / (int64_t(r.blocks) * p->groups) || ns > kMaxGrid * 64) return fail(c, AUD_EINVAL, "tensor too large for one call");
+    if (ni * r.chunks > kMaxGrid / (int64_t(r.blocks) * p->groups) || ns > kMaxGrid * 64 || scan_space(p, r, false).table > kMaxGrid * 256)
+        return fail(c, AUD_EINVAL, "tensor too large for one call");
     const OnDevice device(c);
     AUD_HIP(c, device.err);
     aud::ScanArgs a{};
     fill_scan(p, r, &a);
     a.u = u, a.delta = delta, a.z = z, a.Bm = B, a.Cm = C, a.A = A, a.D = D, a.delta_bias = delta_bias, a.state = state, a.lengths = lengths;
-    a.y = y, a.state_out = state_out, a.kept = kept, a.sums = static_cast<float*>(workspace);
-    if (p->steps == 1 && !kept) {
+    a.y = y, a.state_out = state_out, a.kept = kept, a.table = static_cast<float*>(workspace), a.sums = a.table + scan_space(p, r, false).table;
+    if (p->steps == 1) {
         AUD_HIP(c, aud::launch_scan_step(a, p->dtype, static_cast<hipStream_t>(stream)));
         return AUD_OK;
     }
@@ -393,7 +401,7 @@ int aud_scan_grad_dev(aud_ctx* c, const aud_scan_params* p, const void* dy, cons
     const void* floats[] = {A, D, delta_bias, lengths, kept, dstate_out, dA, dD, ddelta_bias, dstate};
     for (const void* q : floats)
         if (!at(q, 4)) return fail(c, AUD_EINVAL, "pointer not aligned to its type");
-    const aud::ScanRoute r = scan_route_of(p);
+    const aud::ScanRoute r = scan_route_of(p, true);
     int64_t need = 0, kf = 0;
     (void)aud_scan_workspace_bytes(p, 1, &need);
     (void)aud_scan_kept_floats(p, &kf);
@@ -409,16 +417,18 @@ int aud_scan_grad_dev(aud_ctx* c, const aud_scan_params* p, const void* dy, cons
         AUD_HIP(c, aud::launch_column_sums(nullptr, 0, p->channels, p->states, 2, dA, dD, ddelta_bias, static_cast<hipStream_t>(stream)));
         return AUD_OK;
     }
-    if (ni * r.chunks > kMaxGrid / (int64_t(r.blocks) * p->groups) || ns > kMaxGrid * 64 || nbc > kMaxGrid * 64)
+    if (ni * r.chunks > kMaxGrid / (int64_t(r.blocks) * p->groups) || ns > kMaxGrid * 64 || nbc > kMaxGrid * 64 ||
+        scan_space(p, r, true).table > kMaxGrid * 256)
         return fail(c, AUD_EINVAL, "tensor too large for one call");
-    const ScanSpace s = scan_space(p, r);
+    const ScanSpace s = scan_space(p, r, true);
     aud::ScanArgs a{};
     fill_scan(p, r, &a);
     a.u = u, a.delta = delta, a.z = z, a.dy = dy, a.Bm = B, a.Cm = C, a.A = A, a.D = D, a.delta_bias = delta_bias, a.lengths = lengths;
     a.kept = const_cast<float*>(kept);  // (only read)
     a.dstate_out = dstate_out, a.du = du, a.ddelta = ddelta, a.dz = dz, a.dB = dB, a.dC = dC;
     a.dA = dA, a.dD = dD, a.ddelta_bias = ddelta_bias, a.dstate = dstate;
-    a.sums = static_cast<float*>(workspace);
+    a.table = static_cast<float*>(workspace);
+    a.sums = a.table + s.table;
     a.part_bc = a.sums + s.sums;
     a.part = a.part_bc + s.bc;
     const bool aligned = in[0].aligned(4 * e, e) && in[1].aligned(4 * e, e) && in[2].aligned(4 * e, e) && in[3].aligned(4 * e, e) &&

@@ -106,7 +106,7 @@ struct NormArgs {
     const float *weight, *bias;  // [C] or null (1, 0)
     const int32_t* lengths;   // [B] or null
     void* out;                // y or dx, contiguous
-    float* stats;             // [B, G, 2] (mean, 1 / std): out (values), in (gradients)
+    float* stats;             // [B, G, 2] (mean, 1 / std): out (values; may be null), in (gradients)
     float* part;              // workspace, see group_norm.hip
     float *dweight, *dbias;   // [C] or null
     int B, S, C, G;
@@ -115,13 +115,14 @@ struct NormArgs {
     int chunks, chunk_rows;
 };
 struct NormRoute {
-    int vec;     // elements per access: 16 / e, or 1
-    int one_wg;  // > 0: an item fits one workgroup's registers, that many threads; 0: split over `chunks` workgroups
-    int packs;   // ... and that many accesses a thread
+    int vec;                 // elements per access
+    bool one_wg;             // an item in one workgroup; else in `chunks` of chunk_rows rows
     int chunks, chunk_rows;
+    bool join;               // ... whose moments a kernel of its own joins (many groups x chunks)
 };
-NormRoute norm_route(int dtype, int B, int S, int C, bool aligned, bool grad);
-int64_t norm_workspace_floats(const NormRoute& r, int B, int C, int G, bool grad, bool keeps_stats);
+// align: what all addresses and strides are multiples of, bytes
+NormRoute norm_route(int dtype, int B, int S, int C, int G, int align, bool grad);
+int64_t norm_workspace_floats(const NormRoute& r, int B, int C, int G, bool grad);
 hipError_t launch_norm(const NormArgs& a, const NormRoute& r, int dtype, int act, hipStream_t st);
 hipError_t launch_norm_grad(const NormArgs& a, const NormRoute& r, int dtype, int act, hipStream_t st);
 
@@ -158,6 +159,7 @@ struct ScanArgs {
     void *du, *ddelta, *dz;          // [B, L, D] contiguous (dz null: no gate)
     void *dB, *dC;                   // [B, L, G, N] contiguous
     float *dA, *dD, *ddelta_bias, *dstate;  // dD, ddelta_bias, dstate may be null
+    float* table;                    // workspace: B and C in float32 [B, G, 16 tiles, 2, padded states]
     float* sums;                     // workspace: chunk states [B, chunks, N, D], chunk step sums [B, chunks, D]
     float* part_bc;                  // workspace: [2][blocks of a group][B, L, G, N]
     float* part;                     // workspace: [B * chunks][N + 2][D]
@@ -169,7 +171,8 @@ struct ScanRoute {
     int chunks, chunk_tiles;  // the time axis in `chunks` runs of chunk_tiles tiles, scanned side by side and joined
     int blocks;               // blocks of 64 channels a group has
 };
-ScanRoute scan_route(int B, int L, int D, int G, int N);
+int scan_padded_states(int N);
+ScanRoute scan_route(int B, int L, int D, int G, int N, bool grad);
 int64_t scan_sums_floats(const ScanRoute& r, int B, int D, int N);
 hipError_t launch_scan(const ScanArgs& a, const ScanRoute& r, int dtype, bool aligned, hipStream_t st);
 hipError_t launch_scan_step(const ScanArgs& a, int dtype, hipStream_t st);

@@ -8,9 +8,10 @@
 //   g_t = f C_n + carry_t,  du = dt sum_n g B + D f,  ddt = u sum_n g B + sum_n A a h_{t-1} g,  dz = dy v silu'(z)
 //   dB_n = sum_d g dt u,  dC_n = sum_d f h,  dA_n = sum_t dt a h_{t-1} g,  dD = sum f u,  dstate = carry_0
 //
-// A workgroup of four waves owns 64 channels of an item: a lane is a channel, a wave a quarter of the states.  Tiles of 16
-// steps go through LDS: all threads turn u and delta into (dt, dt u), each wave runs its states over the tile, all threads
-// add the four waves' partial sums up and store.
+// A workgroup owns 64 channels of an item: a lane is a channel, a wave a share of the states.  Tiles of 16 steps go through
+// LDS: all threads turn u and delta into (dt, dt u), each wave runs its states over the tile, all threads add the waves'
+// partial sums up and store.  What a step's B and C hold is the same for all lanes of a wave: a small kernel lays them out in
+// float32 first, and the waves read them as scalars, beside the vector pipe and LDS.
 //
 // Where items x channels leave the card idle, the time axis is cut into chunks: (1) every chunk is scanned from a zero state
 // for its final state and its sum of dt, (2) the chunks are joined in order, h' = exp(A sum dt) h + (its final state), (3) every
@@ -24,6 +25,37 @@ namespace {
 
 constexpr int kNT = 256, kT = kScanTile, kCh = 64;
 
+#if defined(__clang__)
+typedef const float __attribute__((address_space(4)))* ScalarTable;  // read by scalar loads: nothing writes it meanwhile
+#else
+typedef const float* ScalarTable;
+#endif
+
+// B and C of GS steps for this wave's NW states, in scalar registers.  The scalar loads of the next group are sent off in front of
+// a group's arithmetic and the LDS reads it needs are done by then: scalar loads come back out of order, so any wait for
+// LDS would wait for them too.
+template <int NW>
+struct Vectors {
+    static constexpr int GS = NW >= 8 ? 2 : 16 / NW < 8 ? 16 / NW : 8;
+    float b[GS][NW], c[GS][NW];
+    template <bool WITH_B, bool WITH_C>
+    __device__ __forceinline__ void load(ScalarTable p) {
+#pragma unroll
+        for (int k = 0; k < GS; ++k)
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                if (WITH_B) b[k][i] = p[k * 2 * NW + i];
+                if (WITH_C) c[k][i] = p[(k * 2 + 1) * NW + i];
+            }
+    }
+};
+
+__device__ __forceinline__ void wait_lds() {  // this wave's LDS reads (and scalar loads) have arrived
+#if defined(__clang__)
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+#endif
+    __builtin_amdgcn_sched_barrier(0);
+}
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 struct Where {  // which channels, chunk and item a workgroup has
@@ -42,56 +74,102 @@ struct Where {  // which channels, chunk and item a workgroup has
     }
 };
 
-// Four channels (c4 .. c4 + 3 of the block) of one step, as float32; channels past the block read as 0
-template <int DT, bool VEC>
-__device__ __forceinline__ void load4(const void* base, int64_t at, int c4, int dn, float (&f)[4]) {
-    if constexpr (VEC) {
-        if (c4 < dn) return unpack<DT, 4>(load_pack<DT, 4>(base, at + c4), f);
+// E neighbouring floats of LDS at once
+template <int E>
+struct alignas(E * 4) Floats {
+    float v[E];
+};
+template <int E>
+__device__ __forceinline__ void lds_read(const float* p, float (&f)[E]) {
+    const Floats<E> q = *reinterpret_cast<const Floats<E>*>(p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = 0.f;
-    } else {
+    for (int i = 0; i < E; ++i) f[i] = q.v[i];
+}
+template <int E>
+__device__ __forceinline__ void lds_write(float* p, const float (&f)[E]) {
+    constexpr int M = E > 4 ? 4 : E;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[i] = c4 + i < dn ? Elem<DT>::up(static_cast<const typename Elem<DT>::raw*>(base)[at + c4 + i]) : 0.f;
+    for (int j = 0; j < E; j += M) {
+        Floats<M> q;
+#pragma unroll
+        for (int i = 0; i < M; ++i) q.v[i] = f[j + i];
+        *reinterpret_cast<Floats<M>*>(p + j) = q;
     }
 }
-template <int DT, bool VEC>
-__device__ __forceinline__ void store4(void* base, int64_t at, int c4, int dn, const float (&f)[4]) {
+// E neighbouring channels of one step as stored, in whole registers: nothing touches them before the step they are wanted in, so
+// the loads stay in flight until then.  Loads are unconditional: the caller gives an address that is there.
+template <int DT, int E, bool VEC>
+struct Raw {
+    static constexpr int S = int(sizeof(typename Elem<DT>::raw));
+    static constexpr bool WHOLE = VEC && E * S >= 4;
+    static constexpr int WORDS = WHOLE ? E * S / 4 : E;
+    struct alignas(WHOLE ? E * S : 4) Words {
+        uint32_t w[WORDS];
+    } r;
+    __device__ __forceinline__ void load(const void* base, int64_t at, int c, int dn) {
+        const typename Elem<DT>::raw* p = static_cast<const typename Elem<DT>::raw*>(base) + at;
+        if constexpr (WHOLE) r = *reinterpret_cast<const Words*>(p + (c < dn ? c : 0));
+        else
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                if constexpr (S == 4) r.w[i] = __float_as_uint(p[c + i < dn ? c + i : 0]);
+                else r.w[i] = p[c + i < dn ? c + i : 0];
+            }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (S == 4) return __uint_as_float(r.w[i]);
+        else if constexpr (WHOLE) return Elem<DT>::up(typename Elem<DT>::raw(i & 1 ? r.w[i / 2] >> 16 : r.w[i / 2] & 0xFFFFu));
+        else return Elem<DT>::up(typename Elem<DT>::raw(r.w[i]));
+    }
+};
+template <int DT, int E, bool VEC>
+__device__ __forceinline__ void store_some(void* base, int64_t at, int c, int dn, const float (&f)[E]) {
     if constexpr (VEC) {
-        if (c4 < dn) store_pack<DT, 4>(base, at + c4, f);
+        if (c < dn) store_pack<DT, E>(base, at + c, f);
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c4 + i < dn) static_cast<typename Elem<DT>::raw*>(base)[at + c4 + i] = Elem<DT>::down(f[i]);
+        for (int i = 0; i < E; ++i)
+            if (c + i < dn) static_cast<typename Elem<DT>::raw*>(base)[at + c + i] = Elem<DT>::down(f[i]);
     }
 }
 
-// dt of a step and its slope d dt / d delta
 __device__ __forceinline__ float step_size(float raw, int softp) { return softp ? softplus(raw) : raw; }
 
-// B or C of a tile -> dst [16][NP] float32; states past N and steps past the tile read as 0
-template <int DT, int NP>
-__device__ __forceinline__ void stage_states(const void* base, int64_t item, int64_t row, int N, int t0, int steps, float* dst) {
-    for (int i = threadIdx.x; i < kT * NP; i += kNT) {
-        const int t = i / NP, n = i % NP;
-        dst[i] = t < steps && n < N ? Elem<DT>::up(static_cast<const typename Elem<DT>::raw*>(base)[item + int64_t(t0 + t) * row + n]) : 0.f;
-    }
+// B and C in float32 -> table [B, G, tiles, waves, 16 steps, B or C, NW states]: what a wave reads of a tile is one run.  States
+// past N and steps at and behind the item's length are 0.
+template <int DT>
+__global__ void __launch_bounds__(kNT) k_scan_table(ScanArgs a, int NP, int NW, int tiles) {
+    const int64_t i = int64_t(blockIdx.x) * kNT + threadIdx.x;
+    const unsigned per = 2 * kT * NP, r = unsigned(i % per);
+    const int n = int(r / (2 * kT * NW) * NW + r % NW), which = int(r / NW % 2);
+    int64_t q = i / per;
+    const int t = int(q % tiles) * kT + int(r / (2 * NW) % kT);
+    q /= tiles;
+    const int g = int(q % a.G);
+    const int64_t b = q / a.G;
+    if (b >= a.B) return;
+    float v = 0.f;
+    if (n < a.N && t < item_rows(a.lengths, int(b), a.L))
+        v = which ? Elem<DT>::up(static_cast<const typename Elem<DT>::raw*>(a.Cm)[b * a.ci + int64_t(t) * a.cr + g * a.N + n])
+                  : Elem<DT>::up(static_cast<const typename Elem<DT>::raw*>(a.Bm)[b * a.bi + int64_t(t) * a.br + g * a.N + n]);
+    a.table[i] = v;
 }
 
-// ---- values.  PASS 1: a chunk's final state from zero and its sum of dt; PASS 3: y ------------------------------------
-template <int DT, int NW, bool VEC, int PASS>
-__global__ void __launch_bounds__(kNT) k_scan(ScanArgs a, int blocks) {
-    constexpr int NP = 4 * NW;
+// ---- values.  PASS 1: a chunk's final state from zero and its sum of dt; PASS 3: y.  W waves of NW states each ---------------
+// One barrier a tile: between two of them a wave runs its states over tile k, turns the inputs of tile k + 1 (on their way
+// while it ran) into steps and, at the next one's start, adds up and stores tile k.  Eight waves of two states (16 states)
+// against four of four: 190 / 275 us at 8 x 2048 x 1536, 16 waves of one: 199.
+template <int DT, int NW, int W, bool VEC, int PASS>
+__global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
+    constexpr int NP = W * NW, E = 16 / W, ROW = kCh / E;  // elements a thread loads and stores, threads a step
     float* lds = reinterpret_cast<float*>(dyn_lds());
-    float2* s_step = reinterpret_cast<float2*>(lds);  // [16][64] (dt, dt u)
-    float* s_b = lds + 2 * kT * kCh;                  // [16][NP]
-    float* s_c = s_b + kT * NP;
-    float* s_y = s_c + kT * NP;                       // [4][16][64]
+    float2* s_step = reinterpret_cast<float2*>(lds);  // [2][16][64] (dt, dt u)
+    float* s_y = lds + 4 * kT * kCh;                  // [2][W][16][64]
     const Where at(a, blocks);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int pt = tid >> 4, c4 = (tid & 15) * 4;     // this thread's step and channels when the tile is loaded and stored
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int pt = tid / ROW, c = (tid % ROW) * E;    // this thread's step and channels when a tile is loaded and stored
     const int len = item_rows(a.lengths, at.b, a.L), tiles = (a.L + kT - 1) / kT;
-    const int64_t u0 = at.b * a.ui + at.d0, e0 = at.b * a.ei + at.d0, z0 = at.b * a.zi + at.d0;
-    const int64_t b0 = at.b * a.bi + at.g * a.N, c0 = at.b * a.ci + at.g * a.N, y0 = int64_t(at.b) * a.L * a.Dn + at.d0;
+    const int64_t u0 = at.b * a.ui + at.d0, e0 = at.b * a.ei + at.d0, z0 = at.b * a.zi + at.d0, y0 = int64_t(at.b) * a.L * a.Dn + at.d0;
     const int d = at.d0 + lane;
     const bool live = lane < at.dn;
     float A2[NW], h[NW], sum_dt = 0.f;
@@ -106,61 +184,100 @@ __global__ void __launch_bounds__(kNT) k_scan(ScanArgs a, int blocks) {
             else if (a.state) h[i] = a.state[(int64_t(at.b) * a.Dn + d) * a.N + n];
         }
     }
-    float skip[4], bias[4];
+    float skip[E], bias[E];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool there = c4 + i < at.dn;
-        skip[i] = there && a.D ? a.D[at.d0 + c4 + i] : 0.f;
-        bias[i] = there && a.delta_bias ? a.delta_bias[at.d0 + c4 + i] : 0.f;
+    for (int i = 0; i < E; ++i) {
+        const bool there = c + i < at.dn;
+        skip[i] = there && a.D ? a.D[at.d0 + c + i] : 0.f;
+        bias[i] = there && a.delta_bias ? a.delta_bias[at.d0 + c + i] : 0.f;
     }
     const int first = at.chunk * a.chunk_tiles, end = first + a.chunk_tiles < tiles ? first + a.chunk_tiles : tiles;
-    for (int tile = first; tile < end; ++tile) {
-        const int t0 = tile * kT, t = t0 + pt;
-        float u[4], dl[4], z[4];
-        if (t < a.L) {
-            load4<DT, VEC>(a.u, u0 + int64_t(t) * a.ur, c4, at.dn, u);
-            load4<DT, VEC>(a.delta, e0 + int64_t(t) * a.er, c4, at.dn, dl);
-            if (PASS == 3 && a.z) load4<DT, VEC>(a.z, z0 + int64_t(t) * a.zr, c4, at.dn, z);
-        }
+    Raw<DT, E, VEC> ru{}, rd{}, rz{};
+    const void* zp = a.z ? a.z : a.u;  // (no gate: read and not used)
+    const int64_t zr = a.z ? a.zr : a.ur, zb = a.z ? z0 : u0;
+    auto fetch = [&](int tile) {
+        const int64_t t = tile * kT + pt < a.L ? tile * kT + pt : a.L - 1;
+        ru.load(a.u, u0 + t * a.ur, c, at.dn);
+        rd.load(a.delta, e0 + t * a.er, c, at.dn);
+        if (PASS == 3) rz.load(zp, zb + t * zr, c, at.dn);
+    };
+    float u[E], z[E];  // of the tile that is being scanned
+    auto stage = [&](int tile, int buf) {
+        float step[2 * E];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool on = t < len;
-            const float dt = on ? step_size(dl[i] + bias[i], a.softplus) : 0.f;
-            s_step[pt * kCh + c4 + i] = float2{dt, on ? dt * u[i] : 0.f};
+        for (int i = 0; i < E; ++i) {
+            const bool on = tile * kT + pt < len && c + i < at.dn;
+            u[i] = on ? ru.get(i) : 0.f;
+            z[i] = on ? rz.get(i) : 0.f;
+            const float dt = on ? step_size(rd.get(i) + bias[i], a.softplus) : 0.f;
+            step[2 * i] = dt;
+            step[2 * i + 1] = dt * u[i];
         }
-        const int steps = len - t0;  // (may be negative)
-        stage_states<DT, NP>(a.Bm, b0, a.br, a.N, t0, steps, s_b);
-        if (PASS == 3) stage_states<DT, NP>(a.Cm, c0, a.cr, a.N, t0, steps, s_c);
+        lds_write(lds + 2 * ((buf * kT + pt) * kCh + c), step);
+    };
+    if (first < end) {
+        fetch(first);
+        stage(first, 0);
+    }
+    __syncthreads();
+    ScalarTable bc = (ScalarTable)(a.table + ((int64_t(at.b) * a.G + at.g) * tiles + first) * kT * 2 * NP + wave * kT * 2 * NW);
+    typedef Vectors<NW> Vec;
+    constexpr int GS = Vec::GS;
+    Vec next{};
+    if (first < end) next.template load<true, PASS == 3>(bc);
+    for (int tile = first, buf = 0; tile < end; ++tile, buf ^= 1, bc += kT * 2 * NP) {
+        if (tile + 1 < end) fetch(tile + 1);
         if (PASS == 3 && a.kept && live) {
 #pragma unroll
             for (int i = 0; i < NW; ++i)
                 if (wave * NW + i < a.N) a.kept[((int64_t(at.b) * tiles + tile) * a.N + wave * NW + i) * a.Dn + d] = h[i];
         }
-        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kT; ++k) {
-            const float2 s = s_step[k * kCh + lane];
-            float y = 0.f;
+        for (int k0 = 0; k0 < kT; k0 += GS) {
+            const Vec now = next;
+            float2 st[GS];
 #pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                h[i] = fmaf(exp2_hw(s.x * A2[i]), h[i], s.y * s_b[k * NP + wave * NW + i]);
-                if (PASS == 3) y = fmaf(s_c[k * NP + wave * NW + i], h[i], y);
+            for (int k = 0; k < GS; ++k) st[k] = s_step[(buf * kT + k0 + k) * kCh + lane];
+            ScalarTable ahead = bc + (k0 + GS) * 2 * NW;
+            if (k0 + GS == kT) ahead = tile + 1 < end ? bc + kT * 2 * NP : bc;  // (nothing behind the last tile: any address of the table)
+            wait_lds();
+            next.template load<true, PASS == 3>(ahead);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < GS; ++k) {
+                float y = 0.f;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) {
+                    h[i] = fmaf(exp2_hw(st[k].x * A2[i]), h[i], st[k].y * now.b[k][i]);
+                    if (PASS == 3) y = fmaf(now.c[k][i], h[i], y);
+                }
+                if (PASS == 3) s_y[((buf * W + wave) * kT + k0 + k) * kCh + lane] = y;
+                else sum_dt += st[k].x;
             }
-            if (PASS == 3) s_y[(wave * kT + k) * kCh + lane] = y;
-            else sum_dt += s.x;
         }
-        __syncthreads();
-        if (PASS == 3 && t < a.L) {
-            float y[4];
+        float su[E], sz[E];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float* p = s_y + pt * kCh + c4 + i;
-                float v = (p[0] + p[kT * kCh]) + (p[2 * kT * kCh] + p[3 * kT * kCh]);
-                v = fmaf(skip[i], u[i], v);
-                if (a.z) v *= z[i] * fast_sigmoid(z[i]);
-                y[i] = t < len ? v : 0.f;
+        for (int i = 0; i < E; ++i) su[i] = u[i], sz[i] = z[i];
+        if (tile + 1 < end) stage(tile + 1, buf ^ 1);
+        __syncthreads();
+        const int t = tile * kT + pt;
+        if (PASS == 3 && t < a.L) {
+            float y[E];
+#pragma unroll
+            for (int i = 0; i < E; ++i) y[i] = skip[i] * su[i];
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                float part[E];
+                lds_read(s_y + ((buf * W + w) * kT + pt) * kCh + c, part);
+#pragma unroll
+                for (int i = 0; i < E; ++i) y[i] += part[i];
             }
-            store4<DT, VEC>(a.y, y0 + int64_t(t) * a.Dn, c4, at.dn, y);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                if (a.z) y[i] *= sz[i] * fast_sigmoid(sz[i]);
+                if (t >= len) y[i] = 0.f;
+            }
+            store_some<DT, E, VEC>(a.y, y0 + int64_t(t) * a.Dn, c, at.dn, y);
         }
     }
     if (!live) return;
@@ -176,9 +293,10 @@ __global__ void __launch_bounds__(kNT) k_scan(ScanArgs a, int blocks) {
 }
 
 // the chunks joined in order: sums[chunk] <- the state in front of it.  BACK: from the last chunk to the first, for the
-// gradient that a chunk receives from behind
+// gradient that a chunk receives from behind.  Eight chunks are read at once, so that their loads wait for one another once.
 template <bool BACK>
 __global__ void __launch_bounds__(kNT) k_scan_join(ScanArgs a) {
+    constexpr int kAhead = 8;
     const int64_t i = int64_t(blockIdx.x) * kNT + threadIdx.x, per = int64_t(a.N) * a.Dn;
     if (i >= a.B * per) return;
     const int64_t b = i / per;
@@ -189,11 +307,21 @@ __global__ void __launch_bounds__(kNT) k_scan_join(ScanArgs a) {
     const int64_t own = (b * a.Dn + d) * a.N + n;
     const float* in = BACK ? a.dstate_out : a.state;
     float h = in ? in[own] : 0.f;
-    for (int k = 0; k < a.chunks; ++k) {
-        const int c = BACK ? a.chunks - 1 - k : k;
-        const float mine = s[c * per];
-        s[c * per] = h;
-        h = fmaf(exp2_hw(dt[int64_t(c) * a.Dn] * A2), h, mine);
+    for (int k = 0; k < a.chunks; k += kAhead) {
+        float mine[kAhead], decay[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int kk = k + j < a.chunks ? k + j : a.chunks - 1, c = BACK ? a.chunks - 1 - kk : kk;
+            mine[j] = s[c * per];
+            decay[j] = dt[int64_t(c) * a.Dn];
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (k + j >= a.chunks) break;
+            const int c = BACK ? a.chunks - 1 - (k + j) : k + j;
+            s[c * per] = h;
+            h = fmaf(exp2_hw(decay[j] * A2), h, mine[j]);
+        }
     }
     float* out = BACK ? a.dstate : a.state_out;
     if (out) out[own] = h;
@@ -217,6 +345,7 @@ __global__ void __launch_bounds__(kNT) k_scan_step(ScanArgs a) {
         for (int n = part; n < a.N; n += 4) {
             const int64_t at = ch * a.N + n;
             float h = a.state ? a.state[at] : 0.f;
+            if (a.kept) a.kept[(b * a.N + n) * a.Dn + d] = h;
             if (live) {
                 const float bn = Elem<DT>::up(static_cast<const raw*>(a.Bm)[b * a.bi + g * a.N + n]);
                 const float cn = Elem<DT>::up(static_cast<const raw*>(a.Cm)[b * a.ci + g * a.N + n]);
@@ -237,25 +366,104 @@ __global__ void __launch_bounds__(kNT) k_scan_step(ScanArgs a) {
     }
 }
 
-// ---- gradients.  PASS 1: what a chunk hands to the one in front of it, from a zero carry, and its sum of dt; PASS 3: all ----
+// ---- gradients ------------------------------------------------------------------------------------------------------------
+// Sums over the 64 lanes of many values at once: two values are joined into one register, each half of the lanes going on
+// with one of them, so 64 values cost 63 additions and leave lane l with the sum of one.  LEVEL 0 .. 5 splits by lane bit
+// 5 - LEVEL; lanes with the bit clear keep `a`.
+template <int LEVEL>
+__device__ __forceinline__ float lane_partner(float v) {
+    constexpr int ctrl = LEVEL == 2 ? 0x140 : LEVEL == 3 ? 0x141 : LEVEL == 4 ? 0x4E : 0xB1;  // l ^ 15, l ^ 7, l ^ 2, l ^ 1
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, 0xF, 0xF, true));
+}
+template <int LEVEL>
+__device__ __forceinline__ float lane_join(float a, float b, int lane) {
+#if defined(__clang__)
+    if constexpr (LEVEL == 0) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else if constexpr (LEVEL == 1) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#else
+    if constexpr (LEVEL < 2) return ((lane >> (5 - LEVEL)) & 1 ? b : a) + __shfl_xor((lane >> (5 - LEVEL)) & 1 ? a : b, 32 >> LEVEL);
+#endif
+    else {
+        const bool up = (lane >> (5 - LEVEL)) & 1;
+        return (up ? b : a) + lane_partner<LEVEL>(up ? a : b);
+    }
+}
+__device__ __forceinline__ float lane_join_at(int level, float a, float b, int lane) {  // (level is a constant where it is called)
+    switch (level) {
+        case 0: return lane_join<0>(a, b, lane);
+        case 1: return lane_join<1>(a, b, lane);
+        case 2: return lane_join<2>(a, b, lane);
+        case 3: return lane_join<3>(a, b, lane);
+        case 4: return lane_join<4>(a, b, lane);
+        default: return lane_join<5>(a, b, lane);
+    }
+}
+constexpr int log2_of(int v) { return v <= 1 ? 0 : 1 + log2_of(v / 2); }
+// The sums over the lanes of v[step][state] for TS steps of NW states, handed in step by step from the last to the first.
+// When step 0 is in, lane l has the sum of state i, step k:  bit q of i = bit 5 - q of l,  bit j of k = bit 5 - log2 NW - j.
+template <int NW, int TS>
+struct LaneSums {
+    static constexpr int LI = log2_of(NW), LK = log2_of(TS), USED = LI + LK;
+    static_assert(USED <= 6, "at most 64 values");
+    float stack[LK > 0 ? LK : 1];
+    float total;
+    __device__ __forceinline__ void add(int k, float (&v)[NW], int lane) {
+#pragma unroll
+        for (int q = 0; q < LI; ++q)
+#pragma unroll
+            for (int i = 0; i < (NW >> (q + 1)); ++i) v[i] = lane_join_at(q, v[2 * i], v[2 * i + 1], lane);
+        float x = v[0];
+#pragma unroll
+        for (int j = 0; j < LK; ++j) {
+            if ((k >> j) & 1) {
+                stack[j] = x;
+                return;
+            }
+            x = lane_join_at(LI + j, x, stack[j], lane);
+        }
+        if constexpr (USED <= 4) x += lane_partner<4>(x);
+        if constexpr (USED <= 5) x += lane_partner<5>(x);
+        total = x;
+    }
+    static __device__ __forceinline__ int state_of(int lane) {
+        int i = 0;
+#pragma unroll
+        for (int q = 0; q < LI; ++q) i |= ((lane >> (5 - q)) & 1) << q;
+        return i;
+    }
+    static __device__ __forceinline__ int step_of(int lane) {
+        int k = 0;
+#pragma unroll
+        for (int j = 0; j < LK; ++j) k |= ((lane >> (5 - LI - j)) & 1) << j;
+        return k;
+    }
+    static __device__ __forceinline__ bool first_of(int lane) { return (lane & ((1 << (6 - USED)) - 1)) == 0; }
+};
+
+// PASS 1: what a chunk hands to the one in front of it, from a zero carry, and its sum of dt; PASS 3: everything.  Four waves
+// of NW states each.
 template <int DT, int NW, bool VEC, int PASS>
-__global__ void __launch_bounds__(kNT) k_scan_grad(ScanArgs a, int blocks) {
-    constexpr int NP = 4 * NW, TS = NW <= 4 ? 16 : 64 / NW, SUBS = kT / TS;  // steps whose states are in registers at once
+__global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
+    constexpr int W = 4, NP = W * NW, E = 4, ROW = kCh / E;
+    constexpr int TS = NW <= 4 ? 16 : 64 / NW, SUBS = kT / TS;  // steps whose states are in registers at once
     float* lds = reinterpret_cast<float*>(dyn_lds());
     float* s_dt = lds;                      // [16][64] each
-    float* s_du = s_dt + kT * kCh;          // dt u
-    float* s_f = s_du + kT * kCh;
-    float* s_b = s_f + kT * kCh;            // [16][NP] each
-    float* s_c = s_b + kT * NP;
-    float* s_db = s_c + kT * NP;
+    float* s_f = s_dt + kT * kCh;
+    float* s_du = s_f + kT * kCh;           // dt u
+    float* s_db = s_du + kT * kCh;          // [16][NP] each
     float* s_dc = s_db + kT * NP;
     float* s_sum = s_dc + kT * NP;          // [3][4][16][64]: sum_n g B, sum_n A a h g, sum_n C h of each wave
     const Where at(a, blocks);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int pt = tid >> 4, c4 = (tid & 15) * 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int pt = tid / ROW, c = (tid % ROW) * E;
     const int len = item_rows(a.lengths, at.b, a.L), tiles = (a.L + kT - 1) / kT;
     const int64_t u0 = at.b * a.ui + at.d0, e0 = at.b * a.ei + at.d0, z0 = at.b * a.zi + at.d0, g0 = at.b * a.yi + at.d0;
-    const int64_t b0 = at.b * a.bi + at.g * a.N, c0 = at.b * a.ci + at.g * a.N, o0 = int64_t(at.b) * a.L * a.Dn + at.d0;
+    const int64_t o0 = int64_t(at.b) * a.L * a.Dn + at.d0;
     const int d = at.d0 + lane;
     const bool live = lane < at.dn;
     float A2[NW], An[NW], carry[NW], dA[NW], sum_dt = 0.f;
@@ -271,145 +479,209 @@ __global__ void __launch_bounds__(kNT) k_scan_grad(ScanArgs a, int blocks) {
             else if (a.dstate_out) carry[i] = a.dstate_out[(int64_t(at.b) * a.Dn + d) * a.N + n];
         }
     }
-    float skip[4], bias[4], sum_fu[4] = {0.f, 0.f, 0.f, 0.f}, sum_dd[4] = {0.f, 0.f, 0.f, 0.f};
+    float skip[E], bias[E], sum_fu[E] = {0.f, 0.f, 0.f, 0.f}, sum_dd[E] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool there = c4 + i < at.dn;
-        skip[i] = there && a.D ? a.D[at.d0 + c4 + i] : 0.f;
-        bias[i] = there && a.delta_bias ? a.delta_bias[at.d0 + c4 + i] : 0.f;
+    for (int i = 0; i < E; ++i) {
+        const bool there = c + i < at.dn;
+        skip[i] = there && a.D ? a.D[at.d0 + c + i] : 0.f;
+        bias[i] = there && a.delta_bias ? a.delta_bias[at.d0 + c + i] : 0.f;
     }
     const int first = at.chunk * a.chunk_tiles, end = first + a.chunk_tiles < tiles ? first + a.chunk_tiles : tiles;
-    for (int tile = end - 1; tile >= first; --tile) {
-        const int t0 = tile * kT, t = t0 + pt, steps = len - t0;
+    Raw<DT, E, VEC> ru{}, rd{}, rz{}, ry{};
+    const void* zp = a.z ? a.z : a.delta;  // (no gate: read and not used)
+    const int64_t zr = a.z ? a.zr : a.er, zb = a.z ? z0 : e0;
+    float h0[NW];  // the state in front of the tile
+    auto fetch = [&](int tile) {
+        const int64_t t = tile * kT + pt < a.L ? tile * kT + pt : a.L - 1;
+        if (PASS == 3) ru.load(a.u, u0 + t * a.ur, c, at.dn);
+        rd.load(a.delta, e0 + t * a.er, c, at.dn);
+        rz.load(zp, zb + t * zr, c, at.dn);
+        ry.load(a.dy, g0 + t * a.yr, c, at.dn);
+        if (PASS == 3)
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                const int n = wave * NW + i;
+                h0[i] = live && n < a.N ? a.kept[((int64_t(at.b) * tiles + tile) * a.N + n) * a.Dn + d] : 0.f;
+            }
+    };
+    if (first < end) fetch(end - 1);
+    ScalarTable bc = (ScalarTable)(a.table + ((int64_t(at.b) * a.G + at.g) * tiles + (end - 1)) * kT * 2 * NP + wave * kT * 2 * NW);
+    for (int tile = end - 1; tile >= first; --tile, bc -= kT * 2 * NP) {
+        const int t0 = tile * kT, t = t0 + pt;
         const bool on = t < len;
-        float u[4], dl[4], z[4], dy[4], dt[4], f[4];
-        if (on) {
-            if (PASS == 3) load4<DT, VEC>(a.u, u0 + int64_t(t) * a.ur, c4, at.dn, u);
-            load4<DT, VEC>(a.delta, e0 + int64_t(t) * a.er, c4, at.dn, dl);
-            if (a.z) load4<DT, VEC>(a.z, z0 + int64_t(t) * a.zr, c4, at.dn, z);
-            load4<DT, VEC>(a.dy, g0 + int64_t(t) * a.yr, c4, at.dn, dy);
-        }
+        float u[E], z[E], dy[E], raw[E], dt[E], f[E], dtu[E], hs0[NW];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (!on) u[i] = dl[i] = z[i] = dy[i] = 0.f;
-            if (PASS == 1) u[i] = 0.f;
-            dt[i] = on ? step_size(dl[i] + bias[i], a.softplus) : 0.f;
+        for (int i = 0; i < E; ++i) {
+            const bool there = on && c + i < at.dn;
+            u[i] = there ? ru.get(i) : 0.f;
+            z[i] = there ? rz.get(i) : 0.f;
+            dy[i] = there ? ry.get(i) : 0.f;
+            raw[i] = (there ? rd.get(i) : 0.f) + bias[i];
+            dt[i] = there ? step_size(raw[i], a.softplus) : 0.f;
             f[i] = a.z ? dy[i] * (z[i] * fast_sigmoid(z[i])) : dy[i];
-            const int s = pt * kCh + c4 + i;
-            s_dt[s] = dt[i];
-            if (PASS == 3) s_du[s] = dt[i] * u[i];
-            s_f[s] = f[i];
+            dtu[i] = dt[i] * u[i];
         }
-        if (PASS == 3) stage_states<DT, NP>(a.Bm, b0, a.br, a.N, t0, steps, s_b);
-        stage_states<DT, NP>(a.Cm, c0, a.cr, a.N, t0, steps, s_c);
-        float h0[NW];
+        lds_write(s_dt + pt * kCh + c, dt);
+        lds_write(s_f + pt * kCh + c, f);
+        if (PASS == 3) lds_write(s_du + pt * kCh + c, dtu);
 #pragma unroll
-        for (int i = 0; i < NW; ++i) {
-            const int n = wave * NW + i;
-            h0[i] = PASS == 3 && live && n < a.N ? a.kept[((int64_t(at.b) * tiles + tile) * a.N + n) * a.Dn + d] : 0.f;
-        }
+        for (int i = 0; i < NW; ++i) hs0[i] = h0[i];
         __syncthreads();
+        if (tile > first) fetch(tile - 1);
+        typedef Vectors<NW> Vec;
+        constexpr int GS = Vec::GS;
         if constexpr (PASS == 1) {
+            Vec next;
+            next.template load<false, true>(bc + (kT - GS) * 2 * NW);
 #pragma unroll
-            for (int k = kT - 1; k >= 0; --k) {
-                const float s = s_dt[k * kCh + lane], fk = s_f[k * kCh + lane];
-                sum_dt += s;
+            for (int k0 = kT - GS; k0 >= 0; k0 -= GS) {
+                const Vec now = next;
+                float s[GS], fk[GS];
 #pragma unroll
-                for (int i = 0; i < NW; ++i)
-                    carry[i] = exp2_hw(s * A2[i]) * fmaf(fk, s_c[k * NP + wave * NW + i], carry[i]);
+                for (int k = 0; k < GS; ++k) s[k] = s_dt[(k0 + k) * kCh + lane], fk[k] = s_f[(k0 + k) * kCh + lane];
+                wait_lds();
+                if (k0 > 0) next.template load<false, true>(bc + (k0 - GS) * 2 * NW);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = GS - 1; k >= 0; --k) {
+                    sum_dt += s[k];
+#pragma unroll
+                    for (int i = 0; i < NW; ++i) carry[i] = exp2_hw(s[k] * A2[i]) * fmaf(fk[k], now.c[k][i], carry[i]);
+                }
             }
         } else {
+            // (a loop where a part is less than the tile: its steps are then not constants, but the tables' offsets stay small)
+#pragma unroll 1
             for (int sub = SUBS - 1; sub >= 0; --sub) {
+                const int k0 = sub * TS;
                 float h[NW], hs[TS][NW], as[TS][NW];  // states behind and decays of the steps of this part of the tile
 #pragma unroll
-                for (int i = 0; i < NW; ++i) h[i] = h0[i];
+                for (int i = 0; i < NW; ++i) h[i] = hs0[i];
                 if constexpr (SUBS > 1)
-                    for (int k = 0; k < sub * TS; ++k)
+                    for (int k = 0; k < k0; ++k)
 #pragma unroll
                         for (int i = 0; i < NW; ++i)
-                            h[i] = fmaf(exp2_hw(s_dt[k * kCh + lane] * A2[i]), h[i], s_du[k * kCh + lane] * s_b[k * NP + wave * NW + i]);
+                            h[i] = fmaf(exp2_hw(s_dt[k * kCh + lane] * A2[i]), h[i], s_du[k * kCh + lane] * bc[k * 2 * NW + i]);
                 float before[NW];
 #pragma unroll
                 for (int i = 0; i < NW; ++i) before[i] = h[i];
+                Vec next;
+                next.template load<true, true>(bc + k0 * 2 * NW);
 #pragma unroll
-                for (int k = 0; k < TS; ++k) {
-                    const int kk = sub * TS + k;
-                    const float s = s_dt[kk * kCh + lane], x = s_du[kk * kCh + lane];
-                    float v = 0.f;
+                for (int q = 0; q < TS; q += GS) {
+                    const Vec now = next;
+                    float s[GS], x[GS];
 #pragma unroll
-                    for (int i = 0; i < NW; ++i) {
-                        as[k][i] = exp2_hw(s * A2[i]);
-                        h[i] = fmaf(as[k][i], h[i], x * s_b[kk * NP + wave * NW + i]);
-                        hs[k][i] = h[i];
-                        v = fmaf(s_c[kk * NP + wave * NW + i], h[i], v);
+                    for (int k = 0; k < GS; ++k) s[k] = s_dt[(k0 + q + k) * kCh + lane], x[k] = s_du[(k0 + q + k) * kCh + lane];
+                    wait_lds();
+                    if (q + GS < TS) next.template load<true, true>(bc + (k0 + q + GS) * 2 * NW);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int k = 0; k < GS; ++k) {
+                        float v = 0.f;
+#pragma unroll
+                        for (int i = 0; i < NW; ++i) {
+                            as[q + k][i] = exp2_hw(s[k] * A2[i]);
+                            h[i] = fmaf(as[q + k][i], h[i], x[k] * now.b[k][i]);
+                            hs[q + k][i] = h[i];
+                            v = fmaf(now.c[k][i], h[i], v);
+                        }
+                        if (a.z) s_sum[((2 * W + wave) * kT + k0 + q + k) * kCh + lane] = v;
                     }
-                    s_sum[((2 * 4 + wave) * kT + kk) * kCh + lane] = v;
                 }
+                LaneSums<NW, TS> sum_b, sum_c;
+                // (the last group's vectors are still there)
 #pragma unroll
-                for (int k = TS - 1; k >= 0; --k) {
-                    const int kk = sub * TS + k;
-                    const float s = s_dt[kk * kCh + lane], x = s_du[kk * kCh + lane], fk = s_f[kk * kCh + lane];
-                    float gb = 0.f, ahg = 0.f;
+                for (int q = TS - GS; q >= 0; q -= GS) {
+                    const Vec now = next;
+                    float s[GS], x[GS], fk[GS];
 #pragma unroll
-                    for (int i = 0; i < NW; ++i) {
-                        const float g = fmaf(fk, s_c[kk * NP + wave * NW + i], carry[i]);
-                        gb = fmaf(g, s_b[kk * NP + wave * NW + i], gb);
-                        carry[i] = as[k][i] * g;
-                        const float r = carry[i] * (k > 0 ? hs[k > 0 ? k - 1 : 0][i] : before[i]);
-                        ahg = fmaf(An[i], r, ahg);
-                        dA[i] = fmaf(s, r, dA[i]);
-                        float pb = live ? g * x : 0.f, pc = live ? fk * hs[k][i] : 0.f;
-                        for (int m = 1; m < 64; m <<= 1) {
-                            pb += __shfl_xor(pb, m);
-                            pc += __shfl_xor(pc, m);
-                        }
-                        if (lane == 0) {
-                            s_db[kk * NP + wave * NW + i] = pb;
-                            s_dc[kk * NP + wave * NW + i] = pc;
-                        }
+                    for (int k = 0; k < GS; ++k) {
+                        s[k] = s_dt[(k0 + q + k) * kCh + lane], x[k] = s_du[(k0 + q + k) * kCh + lane];
+                        fk[k] = s_f[(k0 + q + k) * kCh + lane];
                     }
-                    s_sum[((0 * 4 + wave) * kT + kk) * kCh + lane] = gb;
-                    s_sum[((1 * 4 + wave) * kT + kk) * kCh + lane] = ahg;
+                    wait_lds();
+                    if (q > 0) next.template load<true, true>(bc + (k0 + q - GS) * 2 * NW);
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int k = GS - 1; k >= 0; --k) {
+                        const int kk = q + k;
+                        float gb = 0.f, ahg = 0.f, pb[NW], pc[NW];
+#pragma unroll
+                        for (int i = 0; i < NW; ++i) {
+                            const float g = fmaf(fk[k], now.c[k][i], carry[i]);
+                            gb = fmaf(g, now.b[k][i], gb);
+                            carry[i] = as[kk][i] * g;
+                            const float r = carry[i] * (kk > 0 ? hs[kk > 0 ? kk - 1 : 0][i] : before[i]);
+                            ahg = fmaf(An[i], r, ahg);
+                            dA[i] = fmaf(s[k], r, dA[i]);
+                            pb[i] = g * x[k];
+                            pc[i] = fk[k] * hs[kk][i];
+                        }
+                        sum_b.add(kk, pb, lane);
+                        sum_c.add(kk, pc, lane);
+                        s_sum[((0 * W + wave) * kT + k0 + kk) * kCh + lane] = gb;
+                        s_sum[((1 * W + wave) * kT + k0 + kk) * kCh + lane] = ahg;
+                    }
+                }
+                typedef LaneSums<NW, TS> Sums;
+                if (Sums::first_of(lane)) {
+                    const int o = (k0 + Sums::step_of(lane)) * NP + wave * NW + Sums::state_of(lane);
+                    s_db[o] = sum_b.total;
+                    s_dc[o] = sum_c.total;
                 }
             }
         }
         __syncthreads();
         if constexpr (PASS == 3) {
+            // (the next tile's steps are written beside this: they are read behind the next barrier only)
             if (t < a.L) {
-                float du[4], dd[4], dz[4];
+                float du[E], dd[E], dz[E], sums[3][E];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float sums[3];
+                for (int k = 0; k < 3; ++k) {
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) {
-                        const float* p = s_sum + (k * 4 * kT + pt) * kCh + c4 + i;
-                        sums[k] = (p[0] + p[kT * kCh]) + (p[2 * kT * kCh] + p[3 * kT * kCh]);
-                    }
-                    const float ddt = fmaf(u[i], sums[0], sums[1]);
-                    du[i] = fmaf(dt[i], sums[0], skip[i] * f[i]);
-                    dd[i] = on ? ddt * (a.softplus ? fast_sigmoid(dl[i] + bias[i]) : 1.f) : 0.f;
+                    for (int i = 0; i < E; ++i) sums[k][i] = 0.f;
+                    if (k < 2 || a.z)
+#pragma unroll
+                        for (int w = 0; w < W; ++w) {
+                            float part[E];
+                            lds_read(s_sum + ((k * W + w) * kT + pt) * kCh + c, part);
+#pragma unroll
+                            for (int i = 0; i < E; ++i) sums[k][i] += part[i];
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    const float ddt = fmaf(u[i], sums[0][i], sums[1][i]);
+                    du[i] = fmaf(dt[i], sums[0][i], skip[i] * f[i]);
+                    dd[i] = on ? ddt * (a.softplus ? fast_sigmoid(raw[i]) : 1.f) : 0.f;
                     const float q = fast_sigmoid(z[i]);
-                    dz[i] = dy[i] * fmaf(skip[i], u[i], sums[2]) * (q * (1.f + z[i] * (1.f - q)));
+                    dz[i] = dy[i] * fmaf(skip[i], u[i], sums[2][i]) * (q * (1.f + z[i] * (1.f - q)));
                     sum_fu[i] = fmaf(f[i], u[i], sum_fu[i]);
                     sum_dd[i] += dd[i];
                     if (!on) du[i] = dz[i] = 0.f;
                 }
                 const int64_t o = o0 + int64_t(t) * a.Dn;
-                store4<DT, VEC>(a.du, o, c4, at.dn, du);
-                store4<DT, VEC>(a.ddelta, o, c4, at.dn, dd);
-                if (a.dz) store4<DT, VEC>(a.dz, o, c4, at.dn, dz);
+                store_some<DT, E, VEC>(a.du, o, c, at.dn, du);
+                store_some<DT, E, VEC>(a.ddelta, o, c, at.dn, dd);
+                if (a.dz) store_some<DT, E, VEC>(a.dz, o, c, at.dn, dz);
             }
-            // dB, dC of the tile, summed over this block's channels
-            const int64_t table = int64_t(blocks) * a.B * a.L * a.G * a.N;
+            // dB, dC of the tile, summed over this block's channels: partial sums where the group has more blocks
+            const int64_t table = int64_t(a.B) * a.L * a.G * a.N;
             for (int i = tid; i < kT * NP; i += kNT) {
                 const int k = i / NP, n = i % NP;
                 if (n >= a.N || t0 + k >= a.L) continue;
-                const int64_t o = (((int64_t(at.block) * a.B + at.b) * a.L + t0 + k) * a.G + at.g) * a.N + n;
-                const bool there = k < steps;
-                a.part_bc[o] = there ? s_db[i] : 0.f;
-                a.part_bc[table + o] = there ? s_dc[i] : 0.f;
+                const int64_t o = ((int64_t(at.b) * a.L + t0 + k) * a.G + at.g) * a.N + n;
+                const bool there = t0 + k < len;
+                const float vb = there ? s_db[i] : 0.f, vc = there ? s_dc[i] : 0.f;
+                if (blocks == 1) {
+                    static_cast<typename Elem<DT>::raw*>(a.dB)[o] = Elem<DT>::down(vb);
+                    static_cast<typename Elem<DT>::raw*>(a.dC)[o] = Elem<DT>::down(vc);
+                } else {
+                    a.part_bc[at.block * table + o] = vb;
+                    a.part_bc[(blocks + at.block) * table + o] = vc;
+                }
             }
-            __syncthreads();
         }
     }
     if constexpr (PASS == 1) {
@@ -431,13 +703,13 @@ __global__ void __launch_bounds__(kNT) k_scan_grad(ScanArgs a, int blocks) {
             }
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s_dt[pt * kCh + c4 + i] = sum_fu[i];
-            s_du[pt * kCh + c4 + i] = sum_dd[i];
+        for (int i = 0; i < E; ++i) {
+            s_dt[pt * kCh + c + i] = sum_fu[i];
+            s_f[pt * kCh + c + i] = sum_dd[i];
         }
         __syncthreads();
         if (tid < 2 * kCh && lane < at.dn) {
-            const float* p = (wave == 0 ? s_dt : s_du) + lane;
+            const float* p = (wave == 0 ? s_dt : s_f) + lane;
             float s = 0.f;
             for (int k = 0; k < kT; ++k) s += p[k * kCh];
             row[int64_t(a.N + wave) * a.Dn + d] = s;
@@ -457,44 +729,69 @@ __global__ void __launch_bounds__(kNT) k_scan_bc(ScanArgs a, int blocks) {
     static_cast<typename Elem<DT>::raw*>(i < n ? a.dB : a.dC)[o] = Elem<DT>::down(s);
 }
 
+template <typename K>
+hipError_t allow_lds(K kernel, size_t bytes) {
+    if (bytes <= 64 * 1024) return hipSuccess;
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+}
+
+template <int DT>
+void run_table(const ScanArgs& a, int NP, int NW, hipStream_t st) {
+    const int tiles = (a.L + kT - 1) / kT;
+    const int64_t n = int64_t(a.B) * a.G * tiles * kT * 2 * NP;
+    if (n > 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_table<DT>), dim3(unsigned((n + kNT - 1) / kNT)), dim3(kNT), 0, st, a, NP, NW, tiles);
+}
+template <int DT, int NW, int W, bool VEC>
+hipError_t run(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
+    const dim3 grid(unsigned(int64_t(a.B) * a.chunks * a.G * r.blocks)), wg(64 * W);
+    const size_t lds1 = size_t(4) * kT * kCh * 4, lds3 = lds1 + size_t(2) * W * kT * kCh * 4;
+    if (hipError_t e = allow_lds(&k_scan<DT, NW, W, VEC, 3>, lds3)) return e;
+    run_table<DT>(a, NW * W, NW, st);
+    if (a.chunks > 1) {
+        const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kNT - 1) / kNT);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 1>), grid, wg, lds1, st, a, r.blocks);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<false>), dim3(join), dim3(kNT), 0, st, a);
+    }
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 3>), grid, wg, lds3, st, a, r.blocks);
+    return hipGetLastError();
+}
 template <int DT, int NW, bool VEC>
-hipError_t run(const ScanArgs& a, const ScanRoute& r, bool grad, hipStream_t st) {
+hipError_t run_grad(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     constexpr int NP = 4 * NW;
     const dim3 grid(unsigned(int64_t(a.B) * a.chunks * a.G * r.blocks));
-    const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kNT - 1) / kNT);
-    if (!grad) {
-        const size_t lds = size_t(2 * kT * kCh + 2 * kT * NP + 4 * kT * kCh) * 4;
-        if (a.chunks > 1) {
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, VEC, 1>), grid, dim3(kNT), lds, st, a, r.blocks);
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<false>), dim3(join), dim3(kNT), 0, st, a);
-        }
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, VEC, 3>), grid, dim3(kNT), lds, st, a, r.blocks);
-        return hipGetLastError();
-    }
-    const size_t lds = size_t(3 * kT * kCh + 4 * kT * NP + 12 * kT * kCh) * 4;
-    if (lds > 64 * 1024) {
-        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_scan_grad<DT, NW, VEC, 3>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)) return e;
-        if (hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_scan_grad<DT, NW, VEC, 1>),
-                                               hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024)) return e;
-    }
+    const size_t lds1 = size_t(2) * kT * kCh * 4, lds3 = size_t(3 * kT * kCh + 2 * kT * NP + 12 * kT * kCh) * 4;
+    if (hipError_t e = allow_lds(&k_scan_grad<DT, NW, VEC, 3>, lds3)) return e;
+    run_table<DT>(a, NP, NW, st);
     if (a.chunks > 1) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 1>), grid, dim3(kNT), lds, st, a, r.blocks);
+        const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kNT - 1) / kNT);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 1>), grid, dim3(kNT), lds1, st, a, r.blocks);
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<true>), dim3(join), dim3(kNT), 0, st, a);
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 3>), grid, dim3(kNT), lds, st, a, r.blocks);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 3>), grid, dim3(kNT), lds3, st, a, r.blocks);
     const int64_t bc = 2 * int64_t(a.B) * a.L * a.G * a.N;
-    if (bc > 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_bc<DT>), dim3(unsigned((bc + kNT - 1) / kNT)), dim3(kNT), 0, st, a, r.blocks);
+    if (bc > 0 && r.blocks > 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_bc<DT>), dim3(unsigned((bc + kNT - 1) / kNT)), dim3(kNT), 0, st, a, r.blocks);
     if (hipError_t e = hipGetLastError()) return e;
     return launch_column_sums(a.part, int64_t(a.B) * a.chunks, a.Dn, a.N, 2, a.dA, a.dD, a.ddelta_bias, st);
 }
 template <int DT, bool VEC>
 hipError_t by_states(const ScanArgs& a, const ScanRoute& r, bool grad, hipStream_t st) {
-    if (a.N <= 4) return run<DT, 1, VEC>(a, r, grad, st);
-    if (a.N <= 8) return run<DT, 2, VEC>(a, r, grad, st);
-    if (a.N <= 16) return run<DT, 4, VEC>(a, r, grad, st);
-    if (a.N <= 32) return run<DT, 8, VEC>(a, r, grad, st);
-    return run<DT, 16, VEC>(a, r, grad, st);
+    const int NP = scan_padded_states(a.N);
+    if (grad) {
+        switch (NP) {
+            case 4: return run_grad<DT, 1, VEC>(a, r, st);
+            case 8: return run_grad<DT, 2, VEC>(a, r, st);
+            case 16: return run_grad<DT, 4, VEC>(a, r, st);
+            case 32: return run_grad<DT, 8, VEC>(a, r, st);
+            default: return run_grad<DT, 16, VEC>(a, r, st);
+        }
+    }
+    switch (NP) {
+        case 4: return run<DT, 1, 4, VEC>(a, r, st);
+        case 8: return run<DT, 1, 8, VEC>(a, r, st);
+        case 16: return run<DT, 2, 8, VEC>(a, r, st);
+        case 32: return run<DT, 4, 8, VEC>(a, r, st);
+        default: return run<DT, 8, 8, VEC>(a, r, st);
+    }
 }
 hipError_t by_type(const ScanArgs& a, const ScanRoute& r, int dtype, bool aligned, bool grad, hipStream_t st) {
     const bool vec = aligned && (a.Dn / a.G) % 4 == 0;
@@ -507,13 +804,19 @@ hipError_t by_type(const ScanArgs& a, const ScanRoute& r, int dtype, bool aligne
 
 }  // namespace
 
-// chunks of the time axis: until there are about 1024 workgroups, four tiles a chunk at least (a cut axis is scanned twice)
-ScanRoute scan_route(int B, int L, int D, int G, int) {
+int scan_padded_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : 64; }
+
+// Chunks of the time axis.  A cut axis is scanned twice, which costs 1.7 times the instructions (the first pass has no C, z and
+// y); an uncut one keeps one workgroup a CU and needs enough of them.  Measured at 2048 steps of 64-channel workgroups
+// (bfloat16, 16 states, MI355X): 192 workgroups 190 us uncut, 217 / 216 / 220 us in 4 / 8 / 16 chunks; 64 workgroups 44 us of
+// kernels in 16 chunks, 46 in 8, 78 in 4.  So: uncut from 170 workgroups on, else about 512 workgroups, chunks of four tiles at
+// least.  The gradients (two workgroups a CU): the same, up to 1024 workgroups.
+ScanRoute scan_route(int B, int L, int D, int G, int, bool grad) {
     ScanRoute r{};
     r.blocks = (D / G + kCh - 1) / kCh;
     const int tiles = L > 0 ? (L + kT - 1) / kT : 1;
-    const int64_t wgs = int64_t(B) * G * r.blocks;
-    int64_t chunks = wgs > 0 ? 1024 / wgs : 1;
+    const int64_t wgs = int64_t(B) * G * r.blocks, want = grad ? 1024 : 512;
+    int64_t chunks = wgs >= (grad ? 400 : 170) ? 1 : (want + wgs - 1) / wgs;
     chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, tiles / 4));
     r.chunk_tiles = int((tiles + chunks - 1) / chunks);
     r.chunks = (tiles + r.chunk_tiles - 1) / r.chunk_tiles;

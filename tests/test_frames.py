@@ -30,9 +30,11 @@ def emu_lib():
 @pytest.fixture
 def emu(emu_lib, monkeypatch):
     """the operators on CPU tensors, their kernels run by the thread emulator"""
-    monkeypatch.setattr(frames, "device_of", lambda t, name: 0)
-    monkeypatch.setattr(frames, "stream_of", lambda index: None)
-    return emu_lib
+    monkeypatch.setattr(frames, "context", lambda x, name: runtime.get_ctx(0))
+    monkeypatch.setattr(frames, "current_stream", lambda index: None)
+    yield emu_lib
+    for plans in (norm._PLANS, scan._CONV_PLANS, scan._SCAN_PLANS):  # (they hold the emulator's context)
+        plans.clear()
 
 
 # ---- values and gradients ------------------------------------------------------------------------------------------------
