@@ -10,7 +10,7 @@
 namespace aud {
 namespace {
 
-constexpr int kNT = 256;
+constexpr int kNT = 256, kBatch = 8, kGradBatch = 4;  // steps whose loads are in flight together
 
 struct Run {  // the run of steps and the pack of channels of this thread
     int64_t b;
@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(kNT) k_conv(ConvArgs a, int tiles) {
         for (int j = 0; j < K - 1; ++j) store_pack<DT, V>(a.state_out, (r.b * (K - 1) + j) * a.D + r.c, keep[j]);
     }
     const int64_t from = r.b * a.xi + r.c, to = r.b * int64_t(a.L) * a.D + r.c;
-    for (int t = r.t0; t < end; ++t) {
-        unpack<DT, V>(load_pack<DT, V>(a.x, from + int64_t(t) * a.xr), win[K - 1]);
+    auto step = [&](int t, const Pack<DT, V>& x) {
+        unpack<DT, V>(x, win[K - 1]);
         float y[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -94,7 +94,16 @@ __global__ void __launch_bounds__(kNT) k_conv(ConvArgs a, int tiles) {
         for (int k = 0; k < K - 1; ++k)
 #pragma unroll
             for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
+    };
+    int t = r.t0;
+    for (; t + kBatch <= end; t += kBatch) {
+        Pack<DT, V> x[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) x[j] = load_pack<DT, V>(a.x, from + int64_t(t + j) * a.xr);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) step(t + j, x[j]);
     }
+    for (; t < end; ++t) step(t, load_pack<DT, V>(a.x, from + int64_t(t) * a.xr));
     float zero[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) zero[i] = 0.f;
@@ -124,15 +133,15 @@ __global__ void __launch_bounds__(kNT) k_conv_grad(ConvArgs a, int tiles) {
 #pragma unroll
         for (int j = 0; j < K - 1; ++j) load_ext<DT, V, K>(a, r.b, r.c, int64_t(r.t0) + j, win[j]);
     }
-    for (int t = r.t0; t < last; ++t) {
+    auto step = [&](int t, const Pack<DT, V>& xt, const Pack<DT, V>& dt) {
 #pragma unroll
         for (int k = K - 1; k > 0; --k)
 #pragma unroll
             for (int i = 0; i < V; ++i) q[k][i] = q[k - 1][i];
         if (t < len) {
             float d[V];
-            unpack<DT, V>(load_pack<DT, V>(a.x, r.b * a.xi + int64_t(t) * a.xr + r.c), win[K - 1]);
-            unpack<DT, V>(load_pack<DT, V>(a.dy, r.b * a.di + int64_t(t) * a.dr + r.c), d);
+            unpack<DT, V>(xt, win[K - 1]);
+            unpack<DT, V>(dt, d);
             const bool own = t < r.t1;  // (the K - 1 steps behind the run are the next one's to sum)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -176,6 +185,21 @@ __global__ void __launch_bounds__(kNT) k_conv_grad(ConvArgs a, int tiles) {
         } else if (r.tile == 0 && a.dstate) {
             store_pack<DT, V>(a.dstate, (r.b * (K - 1) + t) * a.D + r.c, de);
         }
+    };
+    const int64_t xb = r.b * a.xi + r.c, db0 = r.b * a.di + r.c;
+    for (int t = r.t0; t < last; t += kGradBatch) {
+        Pack<DT, V> xs[kGradBatch], ds[kGradBatch];
+#pragma unroll
+        for (int j = 0; j < kGradBatch; ++j) {
+            const int64_t row = t + j < len ? t + j : (len > 0 ? len - 1 : 0);  // (a row that is there; not used behind the length)
+            if (len > 0) {
+                xs[j] = load_pack<DT, V>(a.x, xb + row * a.xr);
+                ds[j] = load_pack<DT, V>(a.dy, db0 + row * a.dr);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kGradBatch; ++j)
+            if (t + j < last) step(t + j, xs[j], ds[j]);
     }
     float* part = a.part + (r.b * tiles + r.tile) * int64_t(K + 1) * a.D + r.c;
 #pragma unroll
@@ -228,12 +252,12 @@ hipError_t by_type(const ConvArgs& a, int dtype, int act, int K, bool aligned, b
 
 }  // namespace
 
-// steps a thread walks: as many as leave the card about 4096 waves, between 8 and 64
+// steps a thread walks: as many as leave the card about 2048 waves, between 8 and 64
 int conv_tile(int dtype, int B, int L, int D, bool aligned, bool) {
     const int e = dtype == AUD_F32 ? 4 : 2;
     const int V = aligned && D % (16 / e) == 0 ? 16 / e : 1;
     int T = 64;
-    while (T > 8 && int64_t(B) * (D / V) * ((L + T - 1) / T) < 64 * 4096) T /= 2;
+    while (T > 8 && int64_t(B) * (D / V) * ((L + T - 1) / T) < 64 * 2048) T /= 2;
     return T;
 }
 

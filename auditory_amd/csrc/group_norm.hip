@@ -565,13 +565,13 @@ NormRoute norm_route(int dtype, int B, int S, int C, int G, int align, bool) {
     const int e = dtype == AUD_F32 ? 4 : 2;
     r.vec = align >= 16 && C % (16 / e) == 0 ? 16 / e : align >= 8 && e == 2 && C % 4 == 0 ? 4 : 1;
     const int64_t bytes = int64_t(S) * C * e;
-    r.one_wg = bytes <= 128 * 1024 || (B >= 1024 && bytes <= 1024 * 1024);
+    r.one_wg = bytes <= 32 * 1024 || (B >= 256 && bytes <= 128 * 1024) || (B >= 1024 && bytes <= 1024 * 1024);
     r.chunks = 1;
     r.chunk_rows = S;
     if (!r.one_wg) {
-        // about a thousand workgroups, at least 16 KB of input each
+        // about a thousand workgroups, at least 8 KB of input each
         int64_t chunks = std::min<int64_t>((1024 + B - 1) / B, kMaxChunks);
-        chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, std::min<int64_t>(S, bytes / 16384)));
+        chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, std::min<int64_t>(S, bytes / 8192)));
         r.chunk_rows = int((S + chunks - 1) / chunks);
         r.chunks = (S + r.chunk_rows - 1) / r.chunk_rows;
     }

@@ -23,7 +23,7 @@
 namespace aud {
 namespace {
 
-constexpr int kNT = 256, kT = kScanTile, kCh = 64;
+constexpr int kNT = 256, kT = kScanTile, kCh = 64, kJoinThreads = 64;
 
 #if defined(__clang__)
 typedef const float __attribute__((address_space(4)))* ScalarTable;  // read by scalar loads: nothing writes it meanwhile
@@ -293,11 +293,11 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
 }
 
 // the chunks joined in order: sums[chunk] <- the state in front of it.  BACK: from the last chunk to the first, for the
-// gradient that a chunk receives from behind.  Eight chunks are read at once, so that their loads wait for one another once.
+// gradient that a chunk receives from behind.  Sixteen chunks are read at once, so that their loads wait for one another once.
 template <bool BACK>
-__global__ void __launch_bounds__(kNT) k_scan_join(ScanArgs a) {
-    constexpr int kAhead = 8;
-    const int64_t i = int64_t(blockIdx.x) * kNT + threadIdx.x, per = int64_t(a.N) * a.Dn;
+__global__ void __launch_bounds__(kJoinThreads) k_scan_join(ScanArgs a) {
+    constexpr int kAhead = 16;
+    const int64_t i = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x, per = int64_t(a.N) * a.Dn;
     if (i >= a.B * per) return;
     const int64_t b = i / per;
     const int n = int(i % per / a.Dn), d = int(i % a.Dn);
@@ -748,9 +748,9 @@ hipError_t run(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     if (hipError_t e = allow_lds(&k_scan<DT, NW, W, VEC, 3>, lds3)) return e;
     run_table<DT>(a, NW * W, NW, st);
     if (a.chunks > 1) {
-        const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kNT - 1) / kNT);
+        const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 1>), grid, wg, lds1, st, a, r.blocks);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<false>), dim3(join), dim3(kNT), 0, st, a);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<false>), dim3(join), dim3(kJoinThreads), 0, st, a);
     }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 3>), grid, wg, lds3, st, a, r.blocks);
     return hipGetLastError();
@@ -763,9 +763,9 @@ hipError_t run_grad(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     if (hipError_t e = allow_lds(&k_scan_grad<DT, NW, VEC, 3>, lds3)) return e;
     run_table<DT>(a, NP, NW, st);
     if (a.chunks > 1) {
-        const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kNT - 1) / kNT);
+        const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 1>), grid, dim3(kNT), lds1, st, a, r.blocks);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<true>), dim3(join), dim3(kNT), 0, st, a);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<true>), dim3(join), dim3(kJoinThreads), 0, st, a);
     }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 3>), grid, dim3(kNT), lds3, st, a, r.blocks);
     const int64_t bc = 2 * int64_t(a.B) * a.L * a.G * a.N;
