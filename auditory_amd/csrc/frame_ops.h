@@ -160,7 +160,7 @@ struct ScanArgs {
     void *dB, *dC;                   // [B, L, G, N] contiguous
     float *dA, *dD, *ddelta_bias, *dstate;  // dD, ddelta_bias, dstate may be null
     float* table;                    // workspace: B and C in float32 [B, G, 16 tiles, 2, padded states]
-    float* sums;                     // workspace: chunk states [B, chunks, N, D], chunk step sums [B, chunks, D]
+    float* sums;                     // workspace: chunk states [B, chunks, N, D] (scan.hip chunk_state), chunk step sums [B, chunks, D]
     float* part_bc;                  // workspace: [2][blocks of a group][B, L, G, N]
     float* part;                     // workspace: [B * chunks][N + 2][D]
     int B, L, Dn, G, N, softplus;

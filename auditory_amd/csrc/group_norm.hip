@@ -199,6 +199,109 @@ __global__ void __launch_bounds__(kItemThreads) k_norm_item(NormArgs a) {
     apply_rows<DT, V, ACT, kItemThreads>(a, b, 0, a.S, rows, stats);
 }
 
+// a small item: its values stay in registers (four packs a thread at most), so it is read once, and the variance is summed around
+// the mean itself
+template <int DT, int V, int ACT>
+__global__ void __launch_bounds__(kItemThreads) k_norm_held(NormArgs a) {
+    constexpr int NT = kItemThreads, R = 4;
+    float* stats = reinterpret_cast<float*>(dyn_lds());  // [G, 2]
+    float* entries = stats + 2 * a.G;                    // [lanes][C]
+    const int b = blockIdx.x, rows = item_rows(a.lengths, b, a.S), packs = a.C / V, cg = a.C / a.G;
+    const Lanes<NT> l(packs, 0);
+    const bool mine = l.r < l.lanes;
+    const int64_t base = int64_t(b) * a.xi + int64_t(l.c) * V;
+    float x[R][V];
+    Pack<DT, V> p[R];
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const int row = l.r + j * l.lanes;
+        if (mine && row < rows) p[j] = load_pack<DT, V>(a.x, base + int64_t(row) * a.xr);
+    }
+    float w[V], sh[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        w[i] = mine && a.weight ? a.weight[l.c * V + i] : 1.f;
+        sh[i] = mine && a.bias ? a.bias[l.c * V + i] : 0.f;
+    }
+    int group[V];
+    {
+        int g = l.c * V / cg, in = l.c * V - g * cg;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            group[i] = g;
+            if (++in == cg) in = 0, ++g;
+        }
+    }
+    const float inv = rows ? 1.f / (float(rows) * float(cg)) : 0.f;
+    float m[V], part[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const bool on = mine && l.r + j * l.lanes < rows;
+        if (on) unpack<DT, V>(p[j], x[j]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            if (!on) x[j][i] = 0.f;
+            part[i] += x[j][i];
+        }
+    }
+    // twice: the sum of every group, by way of LDS -> stats[2 g + which]
+    auto sum_groups = [&](int which) {
+        if (mine) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) entries[l.r * a.C + l.c * V + i] = part[i];
+        }
+        __syncthreads();
+        for_groups<NT>(a.G, [&](int g, int lane, int q, bool there) {
+            const int dr = q / cg, dc = q - dr * cg, r0 = lane / cg;
+            float s = 0.f;
+            for (int r = r0, c = lane - r0 * cg; r < l.lanes;) {
+                s += entries[r * a.C + g * cg + c];
+                r += dr, c += dc;
+                if (c >= cg) c -= cg, ++r;
+            }
+            s = sum_lanes(s, q) * inv;
+            if (there && lane == 0) stats[2 * g + which] = s;
+        });
+        __syncthreads();
+    };
+    sum_groups(0);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        m[i] = mine ? stats[2 * group[i]] : 0.f;
+        part[i] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const bool on = mine && l.r + j * l.lanes < rows;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            x[j][i] -= m[i];
+            part[i] = on ? fmaf(x[j][i], x[j][i], part[i]) : part[i];
+        }
+    }
+    sum_groups(1);
+    if (a.stats)
+        for (int g = threadIdx.x; g < a.G; g += NT) {
+            a.stats[(int64_t(b) * a.G + g) * 2] = stats[2 * g];
+            a.stats[(int64_t(b) * a.G + g) * 2 + 1] = 1.f / sqrtf(stats[2 * g + 1] + a.eps);
+        }
+    if (!mine) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] *= 1.f / sqrtf(stats[2 * group[i] + 1] + a.eps);
+    const int64_t to = int64_t(b) * a.S * a.C + int64_t(l.c) * V;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+        const int row = l.r + j * l.lanes;
+        if (row >= a.S) continue;
+        float y[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) y[i] = row < rows ? act_value<ACT>(fmaf(x[j][i], w[i], sh[i])) : 0.f;
+        store_pack<DT, V>(a.out, to + int64_t(row) * a.C, y);
+    }
+}
+
 // an item over several workgroups: moments of a chunk of rows -> part [B, chunks, G, 2]
 template <int DT, int V>
 __global__ void __launch_bounds__(kChunkThreads) k_norm_chunk(NormArgs a) {
@@ -486,6 +589,13 @@ inline size_t entries_of(int nt, int V, int C) { return size_t(2) * size_t(std::
 
 template <int DT, int V, int ACT>
 hipError_t run(const NormArgs& a, const NormRoute& r, hipStream_t st) {
+    const int packs = a.C / V;
+    if (r.one_wg && packs <= kItemThreads && int64_t(a.S) <= 4 * (kItemThreads / packs)) {
+        const size_t lds = (2 * size_t(a.G) + size_t(kItemThreads / packs) * a.C) * 4;
+        if (hipError_t e = allow_lds(&k_norm_held<DT, V, ACT>, lds)) return e;
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_held<DT, V, ACT>), dim3(unsigned(a.B)), dim3(kItemThreads), lds, st, a);
+        return hipGetLastError();
+    }
     if (r.one_wg) {
         const size_t lds = (2 * size_t(a.G) + entries_of(kItemThreads, V, a.C)) * 4;
         if (hipError_t e = allow_lds(&k_norm_item<DT, V, ACT>, lds)) return e;

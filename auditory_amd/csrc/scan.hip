@@ -13,9 +13,9 @@
 // partial sums up and store.  What a step's B and C hold is the same for all lanes of a wave: a small kernel lays them out in
 // float32 first, and the waves read them as scalars, beside the vector pipe and LDS.
 //
-// Where items x channels leave the card idle, the time axis is cut into chunks: (1) every chunk is scanned from a zero state
-// for its final state and its sum of dt, (2) the chunks are joined in order, h' = exp(A sum dt) h + (its final state), (3) every
-// chunk is scanned from its true state.
+// Where items x channels leave the card idle, the time axis is cut into chunks: (1) every chunk but the last is scanned, the
+// first from the true state, the others from zero, for its final state and its sum of dt; (3) every chunk works its true
+// state out from those, h' = exp(A sum dt) h + (final state) chunk by chunk, and is scanned from there.
 //
 // Steps at and behind lengths[b] have dt = 0: the state stays, y is zero, and what the inputs hold there has no effect.
 #include "frame_ops.h"
@@ -23,7 +23,11 @@
 namespace aud {
 namespace {
 
-constexpr int kNT = 256, kT = kScanTile, kCh = 64, kJoinThreads = 64;
+constexpr int kNT = 256, kT = kScanTile, kCh = 64;
+constexpr int kMaxChunks = 64, kJoinThreads = 64;
+// Up to 8 chunks a workgroup walks the ones in front of its own; with more that reads too much (16 chunks, 64 workgroups of
+// channels: 9 us more in the second scan) and a kernel between the scans (5 us) joins them.
+constexpr int kFoldChunks = 8;
 
 #if defined(__clang__)
 typedef const float __attribute__((address_space(4)))* ScalarTable;  // read by scalar loads: nothing writes it meanwhile
@@ -56,18 +60,27 @@ __device__ __forceinline__ void wait_lds() {  // this wave's LDS reads (and scal
 #endif
     __builtin_amdgcn_sched_barrier(0);
 }
+// Everything loaded so far has arrived.  In front of a loop: a register that is still on its way there would be waited for in
+// every turn, and the loads that the turn has sent off with it.
+__device__ __forceinline__ void wait_loads() {
+#if defined(__clang__)
+    __builtin_amdgcn_s_waitcnt(0x0F70);
+#endif
+}
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 struct Where {  // which channels, chunk and item a workgroup has
     int b, chunk, g, d0, dn, block;  // first channel, channels (<= 64), block within the group
-    __device__ __forceinline__ Where(const ScanArgs& a, int blocks) {
+    // (the first pass leaves the last chunk out, the gradients' first pass the first one)
+    __device__ __forceinline__ Where(const ScanArgs& a, int blocks, int skip_last, int skip_first) {
         int id = blockIdx.x;
         block = id % blocks;
         id /= blocks;
         g = id % a.G;
         id /= a.G;
-        chunk = id % a.chunks;
-        b = id / a.chunks;
+        const int chunks = a.chunks - skip_last - skip_first;
+        chunk = id % chunks + skip_first;
+        b = id / chunks;
         const int dg = a.Dn / a.G;
         d0 = g * dg + block * kCh;
         dn = dg - block * kCh < kCh ? dg - block * kCh : kCh;
@@ -106,14 +119,14 @@ struct Raw {
     struct alignas(WHOLE ? E * S : 4) Words {
         uint32_t w[WORDS];
     } r;
-    __device__ __forceinline__ void load(const void* base, int64_t at, int c, int dn) {
-        const typename Elem<DT>::raw* p = static_cast<const typename Elem<DT>::raw*>(base) + at;
-        if constexpr (WHOLE) r = *reinterpret_cast<const Words*>(p + (c < dn ? c : 0));
+    // p: the first of the channels, `left` of them are there (one at least)
+    __device__ __forceinline__ void load(const typename Elem<DT>::raw* p, int left) {
+        if constexpr (WHOLE) r = *reinterpret_cast<const Words*>(p);
         else
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                if constexpr (S == 4) r.w[i] = __float_as_uint(p[c + i < dn ? c + i : 0]);
-                else r.w[i] = p[c + i < dn ? c + i : 0];
+                if constexpr (S == 4) r.w[i] = __float_as_uint(p[i < left ? i : 0]);
+                else r.w[i] = p[i < left ? i : 0];
             }
     }
     __device__ __forceinline__ float get(int i) const {
@@ -155,6 +168,45 @@ __global__ void __launch_bounds__(kNT) k_scan_table(ScanArgs a, int NP, int NW, 
     a.table[i] = v;
 }
 
+// What a chunk starts from, worked out from the table `sums` of the first pass.  Forward: slot 0 holds the first state, slot c + 1
+// the state behind chunk c as far as the chunk knows it (chunk 0: the true one).  BACK, from the end: slot c + 1 holds what chunk
+// c + 1 hands back (the last one: truly).  Several slots are read at once, so that their loads wait for one another once.
+template <int NW, bool BACK>
+__device__ __forceinline__ void chunk_state(const ScanArgs& a, const Where& at, int n0, int d, bool live, const float (&A2)[NW], float (&h)[NW]) {
+    constexpr int kAhead = NW <= 8 ? kFoldChunks : 4;
+    const int64_t per = int64_t(a.N) * a.Dn;
+    const float* s = a.sums + int64_t(at.b) * a.chunks * per + d;
+    const float* dt = a.sums + int64_t(a.B) * a.chunks * per + int64_t(at.b) * a.chunks * a.Dn + d;
+    if (!live) return;
+    if (a.chunks > kFoldChunks) {  // k_scan_join has been over the table
+        const int64_t slot = BACK ? at.chunk + 1 : at.chunk;
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+            if (n0 + i < a.N) h[i] = s[slot * per + int64_t(n0 + i) * a.Dn];
+        return;
+    }
+    // forward: slots 1 .. chunk (slot 0 alone for chunk 0); back: slots chunks - 1 down to chunk + 1
+    const int count = BACK ? a.chunks - 1 - at.chunk : (at.chunk > 0 ? at.chunk : 1);
+    for (int k = 0; k < count; k += kAhead) {
+        float part[kAhead][NW], sum[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int kk = k + j < count ? k + j : count - 1;
+            const int slot = BACK ? a.chunks - 1 - kk : (at.chunk > 0 ? 1 + kk : 0);
+            const int chunk = BACK ? slot : (slot > 0 ? slot - 1 : 0);
+            sum[j] = dt[int64_t(chunk) * a.Dn];
+#pragma unroll
+            for (int i = 0; i < NW; ++i) part[j][i] = n0 + i < a.N ? s[slot * per + int64_t(n0 + i) * a.Dn] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (k + j >= count) break;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) h[i] = k + j == 0 ? part[j][i] : fmaf(exp2_hw(sum[j] * A2[i]), h[i], part[j][i]);
+        }
+    }
+}
+
 // ---- values.  PASS 1: a chunk's final state from zero and its sum of dt; PASS 3: y.  W waves of NW states each ---------------
 // One barrier a tile: between two of them a wave runs its states over tile k, turns the inputs of tile k + 1 (on their way
 // while it ran) into steps and, at the next one's start, adds up and stores tile k.  Eight waves of two states (16 states)
@@ -165,7 +217,7 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     float* lds = reinterpret_cast<float*>(dyn_lds());
     float2* s_step = reinterpret_cast<float2*>(lds);  // [2][16][64] (dt, dt u)
     float* s_y = lds + 4 * kT * kCh;                  // [2][W][16][64]
-    const Where at(a, blocks);
+    const Where at(a, blocks, PASS == 1, 0);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int pt = tid / ROW, c = (tid % ROW) * E;    // this thread's step and channels when a tile is loaded and stored
     const int len = item_rows(a.lengths, at.b, a.L), tiles = (a.L + kT - 1) / kT;
@@ -179,11 +231,11 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
         const bool there = live && n < a.N;
         A2[i] = there ? a.A[int64_t(d) * a.N + n] * kLog2e : 0.f;
         h[i] = 0.f;
-        if (PASS == 3 && there) {
-            if (a.chunks > 1) h[i] = a.sums[((int64_t(at.b) * a.chunks + at.chunk) * a.N + n) * a.Dn + d];
-            else if (a.state) h[i] = a.state[(int64_t(at.b) * a.Dn + d) * a.N + n];
-        }
+        if (there && at.chunk == 0 && (PASS == 1 || a.chunks == 1) && a.state) h[i] = a.state[(int64_t(at.b) * a.Dn + d) * a.N + n];
+        // (a copy for the first chunk's second scan: state_out, written by the last chunk, may be the state itself)
+        if (there && at.chunk == 0 && PASS == 1) a.sums[(int64_t(at.b) * a.chunks * a.N + n) * a.Dn + d] = h[i];
     }
+    if (PASS == 3 && a.chunks > 1) chunk_state<NW, false>(a, at, wave * NW, d, live, A2, h);
     float skip[E], bias[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -193,14 +245,25 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     }
     const int first = at.chunk * a.chunk_tiles, end = first + a.chunk_tiles < tiles ? first + a.chunk_tiles : tiles;
     Raw<DT, E, VEC> ru{}, rd{}, rz{};
-    const void* zp = a.z ? a.z : a.u;  // (no gate: read and not used)
-    const int64_t zr = a.z ? a.zr : a.ur, zb = a.z ? z0 : u0;
-    auto fetch = [&](int tile) {
-        const int64_t t = tile * kT + pt < a.L ? tile * kT + pt : a.L - 1;
-        ru.load(a.u, u0 + t * a.ur, c, at.dn);
-        rd.load(a.delta, e0 + t * a.er, c, at.dn);
-        if (PASS == 3) rz.load(zp, zb + t * zr, c, at.dn);
+    // addresses of this thread's channels in its row of the tile, moved on by 16 rows a tile (a row behind the last one is not
+    // looked at: the address stays where it is)
+    typedef typename Elem<DT>::raw raw;
+    const int cc = c < at.dn ? c : 0, left = at.dn - cc;
+    const int64_t row = first * kT + pt < a.L ? first * kT + pt : (a.L > 0 ? a.L - 1 : 0);
+    const raw* pu = static_cast<const raw*>(a.u) + u0 + row * a.ur + cc;
+    const raw* pd = static_cast<const raw*>(a.delta) + e0 + row * a.er + cc;
+    const raw* pz = a.z ? static_cast<const raw*>(a.z) + z0 + row * a.zr + cc : pu;  // (no gate: read and not used)
+    const int64_t su = kT * a.ur, sd = kT * a.er, sz_ = a.z ? kT * a.zr : su;
+    auto fetch = [&] {
+        ru.load(pu, left);
+        rd.load(pd, left);
+        if (PASS == 3) rz.load(pz, left);
     };
+    auto advance = [&](int tile) {
+        if (tile * kT + pt < a.L) pu += su, pd += sd, pz += sz_;
+    };
+    float* pk = a.kept ? a.kept + ((int64_t(at.b) * tiles + first) * a.N + wave * NW) * a.Dn + d : nullptr;
+    raw* py = PASS == 3 ? static_cast<raw*>(a.y) + y0 + int64_t(first * kT + pt) * a.Dn : nullptr;
     float u[E], z[E];  // of the tile that is being scanned
     auto stage = [&](int tile, int buf) {
         float step[2 * E];
@@ -216,7 +279,7 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
         lds_write(lds + 2 * ((buf * kT + pt) * kCh + c), step);
     };
     if (first < end) {
-        fetch(first);
+        fetch();
         stage(first, 0);
     }
     __syncthreads();
@@ -224,13 +287,18 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     typedef Vectors<NW> Vec;
     constexpr int GS = Vec::GS;
     Vec next{};
+    wait_loads();
     if (first < end) next.template load<true, PASS == 3>(bc);
     for (int tile = first, buf = 0; tile < end; ++tile, buf ^= 1, bc += kT * 2 * NP) {
-        if (tile + 1 < end) fetch(tile + 1);
-        if (PASS == 3 && a.kept && live) {
+        if (tile + 1 < end) {
+            advance(tile + 1);
+            fetch();
+        }
+        if (PASS == 3 && a.kept) {
 #pragma unroll
             for (int i = 0; i < NW; ++i)
-                if (wave * NW + i < a.N) a.kept[((int64_t(at.b) * tiles + tile) * a.N + wave * NW + i) * a.Dn + d] = h[i];
+                if (live && wave * NW + i < a.N) pk[int64_t(i) * a.Dn] = h[i];
+            pk += int64_t(a.N) * a.Dn;
         }
 #pragma unroll
         for (int k0 = 0; k0 < kT; k0 += GS) {
@@ -277,8 +345,9 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
                 if (a.z) y[i] *= sz[i] * fast_sigmoid(sz[i]);
                 if (t >= len) y[i] = 0.f;
             }
-            store_some<DT, E, VEC>(a.y, y0 + int64_t(t) * a.Dn, c, at.dn, y);
+            store_some<DT, E, VEC>(py, 0, c, at.dn, y);
         }
+        if (PASS == 3) py += kT * a.Dn;
     }
     if (!live) return;
     float* dt_sums = a.sums + int64_t(a.B) * a.chunks * a.N * a.Dn;
@@ -286,45 +355,41 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     for (int i = 0; i < NW; ++i) {
         const int n = wave * NW + i;
         if (n >= a.N) continue;
-        if (PASS == 1) a.sums[((int64_t(at.b) * a.chunks + at.chunk) * a.N + n) * a.Dn + d] = h[i];
-        else if (a.chunks == 1 && a.state_out) a.state_out[(int64_t(at.b) * a.Dn + d) * a.N + n] = h[i];
+        if (PASS == 1) a.sums[((int64_t(at.b) * a.chunks + at.chunk + 1) * a.N + n) * a.Dn + d] = h[i];
+        else if (at.chunk == a.chunks - 1 && a.state_out) a.state_out[(int64_t(at.b) * a.Dn + d) * a.N + n] = h[i];
     }
     if (PASS == 1 && wave == 0) dt_sums[(int64_t(at.b) * a.chunks + at.chunk) * a.Dn + d] = sum_dt;
 }
 
-// the chunks joined in order: sums[chunk] <- the state in front of it.  BACK: from the last chunk to the first, for the
-// gradient that a chunk receives from behind.  Sixteen chunks are read at once, so that their loads wait for one another once.
+// many chunks: the same once for all of them, slot by slot in place (sixteen at once)
 template <bool BACK>
 __global__ void __launch_bounds__(kJoinThreads) k_scan_join(ScanArgs a) {
     constexpr int kAhead = 16;
-    const int64_t i = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x, per = int64_t(a.N) * a.Dn;
-    if (i >= a.B * per) return;
-    const int64_t b = i / per;
-    const int n = int(i % per / a.Dn), d = int(i % a.Dn);
+    const int64_t id = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x, per = int64_t(a.N) * a.Dn;
+    if (id >= a.B * per) return;
+    const int64_t b = id / per;
+    const int n = int(id % per / a.Dn), d = int(id % a.Dn);
     const float A2 = a.A[int64_t(d) * a.N + n] * kLog2e;
     float* s = a.sums + b * a.chunks * per + int64_t(n) * a.Dn + d;
     const float* dt = a.sums + int64_t(a.B) * a.chunks * per + b * a.chunks * a.Dn + d;
-    const int64_t own = (b * a.Dn + d) * a.N + n;
-    const float* in = BACK ? a.dstate_out : a.state;
-    float h = in ? in[own] : 0.f;
-    for (int k = 0; k < a.chunks; k += kAhead) {
-        float mine[kAhead], decay[kAhead];
+    // slots 1 .. chunks - 1, forward from 1 or back from the last; the first of them is true already
+    float h = 0.f;
+    for (int k = 0; k < a.chunks - 1; k += kAhead) {
+        float mine[kAhead], sum[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const int kk = k + j < a.chunks ? k + j : a.chunks - 1, c = BACK ? a.chunks - 1 - kk : kk;
-            mine[j] = s[c * per];
-            decay[j] = dt[int64_t(c) * a.Dn];
+            const int kk = k + j < a.chunks - 1 ? k + j : a.chunks - 2, slot = BACK ? a.chunks - 1 - kk : 1 + kk;
+            mine[j] = s[slot * per];
+            sum[j] = dt[int64_t(BACK ? slot : slot - 1) * a.Dn];
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            if (k + j >= a.chunks) break;
-            const int c = BACK ? a.chunks - 1 - (k + j) : k + j;
-            s[c * per] = h;
-            h = fmaf(exp2_hw(decay[j] * A2), h, mine[j]);
+            if (k + j >= a.chunks - 1) break;
+            const int slot = BACK ? a.chunks - 1 - (k + j) : 1 + k + j;
+            h = k + j == 0 ? mine[j] : fmaf(exp2_hw(sum[j] * A2), h, mine[j]);
+            s[slot * per] = h;
         }
     }
-    float* out = BACK ? a.dstate : a.state_out;
-    if (out) out[own] = h;
 }
 
 // ---- one frame: four lanes a channel, a quarter of its states each ----------------------------------------------------
@@ -458,7 +523,7 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
     float* s_db = s_du + kT * kCh;          // [16][NP] each
     float* s_dc = s_db + kT * NP;
     float* s_sum = s_dc + kT * NP;          // [3][4][16][64]: sum_n g B, sum_n A a h g, sum_n C h of each wave
-    const Where at(a, blocks);
+    const Where at(a, blocks, 0, PASS == 1);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int pt = tid / ROW, c = (tid % ROW) * E;
     const int len = item_rows(a.lengths, at.b, a.L), tiles = (a.L + kT - 1) / kT;
@@ -474,11 +539,9 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
         An[i] = there ? a.A[int64_t(d) * a.N + n] : 0.f;
         A2[i] = An[i] * kLog2e;
         carry[i] = dA[i] = 0.f;
-        if (PASS == 3 && there) {
-            if (a.chunks > 1) carry[i] = a.sums[((int64_t(at.b) * a.chunks + at.chunk) * a.N + n) * a.Dn + d];
-            else if (a.dstate_out) carry[i] = a.dstate_out[(int64_t(at.b) * a.Dn + d) * a.N + n];
-        }
+        if (there && at.chunk == a.chunks - 1 && a.dstate_out) carry[i] = a.dstate_out[(int64_t(at.b) * a.Dn + d) * a.N + n];
     }
+    if (PASS == 3 && at.chunk < a.chunks - 1) chunk_state<NW, true>(a, at, wave * NW, d, live, A2, carry);
     float skip[E], bias[E], sum_fu[E] = {0.f, 0.f, 0.f, 0.f}, sum_dd[E] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -488,15 +551,15 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
     }
     const int first = at.chunk * a.chunk_tiles, end = first + a.chunk_tiles < tiles ? first + a.chunk_tiles : tiles;
     Raw<DT, E, VEC> ru{}, rd{}, rz{}, ry{};
-    const void* zp = a.z ? a.z : a.delta;  // (no gate: read and not used)
-    const int64_t zr = a.z ? a.zr : a.er, zb = a.z ? z0 : e0;
+    typedef typename Elem<DT>::raw raw;
+    const int cc = c < at.dn ? c : 0, left = at.dn - cc;
     float h0[NW];  // the state in front of the tile
     auto fetch = [&](int tile) {
-        const int64_t t = tile * kT + pt < a.L ? tile * kT + pt : a.L - 1;
-        if (PASS == 3) ru.load(a.u, u0 + t * a.ur, c, at.dn);
-        rd.load(a.delta, e0 + t * a.er, c, at.dn);
-        rz.load(zp, zb + t * zr, c, at.dn);
-        ry.load(a.dy, g0 + t * a.yr, c, at.dn);
+        const int64_t row = tile * kT + pt < a.L ? tile * kT + pt : a.L - 1;
+        if (PASS == 3) ru.load(static_cast<const raw*>(a.u) + u0 + row * a.ur + cc, left);
+        rd.load(static_cast<const raw*>(a.delta) + e0 + row * a.er + cc, left);
+        if (a.z) rz.load(static_cast<const raw*>(a.z) + z0 + row * a.zr + cc, left);
+        ry.load(static_cast<const raw*>(a.dy) + g0 + row * a.yr + cc, left);
         if (PASS == 3)
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
@@ -504,20 +567,21 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
                 h0[i] = live && n < a.N ? a.kept[((int64_t(at.b) * tiles + tile) * a.N + n) * a.Dn + d] : 0.f;
             }
     };
+    wait_loads();
     if (first < end) fetch(end - 1);
     ScalarTable bc = (ScalarTable)(a.table + ((int64_t(at.b) * a.G + at.g) * tiles + (end - 1)) * kT * 2 * NP + wave * kT * 2 * NW);
     for (int tile = end - 1; tile >= first; --tile, bc -= kT * 2 * NP) {
         const int t0 = tile * kT, t = t0 + pt;
         const bool on = t < len;
-        float u[E], z[E], dy[E], raw[E], dt[E], f[E], dtu[E], hs0[NW];
+        float u[E], z[E], dy[E], arg[E], dt[E], f[E], dtu[E], hs0[NW];
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const bool there = on && c + i < at.dn;
             u[i] = there ? ru.get(i) : 0.f;
             z[i] = there ? rz.get(i) : 0.f;
             dy[i] = there ? ry.get(i) : 0.f;
-            raw[i] = (there ? rd.get(i) : 0.f) + bias[i];
-            dt[i] = there ? step_size(raw[i], a.softplus) : 0.f;
+            arg[i] = (there ? rd.get(i) : 0.f) + bias[i];
+            dt[i] = there ? step_size(arg[i], a.softplus) : 0.f;
             f[i] = a.z ? dy[i] * (z[i] * fast_sigmoid(z[i])) : dy[i];
             dtu[i] = dt[i] * u[i];
         }
@@ -654,7 +718,7 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
                 for (int i = 0; i < E; ++i) {
                     const float ddt = fmaf(u[i], sums[0][i], sums[1][i]);
                     du[i] = fmaf(dt[i], sums[0][i], skip[i] * f[i]);
-                    dd[i] = on ? ddt * (a.softplus ? fast_sigmoid(raw[i]) : 1.f) : 0.f;
+                    dd[i] = on ? ddt * (a.softplus ? fast_sigmoid(arg[i]) : 1.f) : 0.f;
                     const float q = fast_sigmoid(z[i]);
                     dz[i] = dy[i] * fmaf(skip[i], u[i], sums[2][i]) * (q * (1.f + z[i] * (1.f - q)));
                     sum_fu[i] = fmaf(f[i], u[i], sum_fu[i]);
@@ -699,7 +763,7 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
                 const int n = wave * NW + i;
                 if (n >= a.N) continue;
                 row[int64_t(n) * a.Dn + d] = dA[i];
-                if (a.chunks == 1 && a.dstate) a.dstate[(int64_t(at.b) * a.Dn + d) * a.N + n] = carry[i];
+                if (at.chunk == 0 && a.dstate) a.dstate[(int64_t(at.b) * a.Dn + d) * a.N + n] = carry[i];
             }
         }
 #pragma unroll
@@ -748,9 +812,12 @@ hipError_t run(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     if (hipError_t e = allow_lds(&k_scan<DT, NW, W, VEC, 3>, lds3)) return e;
     run_table<DT>(a, NW * W, NW, st);
     if (a.chunks > 1) {
-        const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 1>), grid, wg, lds1, st, a, r.blocks);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<false>), dim3(join), dim3(kJoinThreads), 0, st, a);
+        const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 1>), first, wg, lds1, st, a, r.blocks);
+        if (a.chunks > kFoldChunks) {
+            const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<false>), dim3(join), dim3(kJoinThreads), 0, st, a);
+        }
     }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 3>), grid, wg, lds3, st, a, r.blocks);
     return hipGetLastError();
@@ -763,9 +830,12 @@ hipError_t run_grad(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     if (hipError_t e = allow_lds(&k_scan_grad<DT, NW, VEC, 3>, lds3)) return e;
     run_table<DT>(a, NP, NW, st);
     if (a.chunks > 1) {
-        const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 1>), grid, dim3(kNT), lds1, st, a, r.blocks);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<true>), dim3(join), dim3(kJoinThreads), 0, st, a);
+        const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 1>), first, dim3(kNT), lds1, st, a, r.blocks);
+        if (a.chunks > kFoldChunks) {
+            const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<true>), dim3(join), dim3(kJoinThreads), 0, st, a);
+        }
     }
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 3>), grid, dim3(kNT), lds3, st, a, r.blocks);
     const int64_t bc = 2 * int64_t(a.B) * a.L * a.G * a.N;
@@ -817,7 +887,7 @@ ScanRoute scan_route(int B, int L, int D, int G, int, bool grad) {
     const int tiles = L > 0 ? (L + kT - 1) / kT : 1;
     const int64_t wgs = int64_t(B) * G * r.blocks, want = grad ? 1024 : 512;
     int64_t chunks = wgs >= (grad ? 400 : 170) ? 1 : (want + wgs - 1) / wgs;
-    chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, tiles / 4));
+    chunks = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(chunks, kMaxChunks), tiles / 4));
     r.chunk_tiles = int((tiles + chunks - 1) / chunks);
     r.chunks = (tiles + r.chunk_tiles - 1) / r.chunk_tiles;
     return r;
