@@ -1,5 +1,9 @@
 """Device-resident batch driver: many utterances as one grid, sharded over the GPUs of a node.
 
+Behind the reference's own stages stand the operators that networks put on their tensors: group norm with an activation
+(group_norm, process_norm; auditory_amd.norm) and, over the frames, a causal convolution and a selective scan
+(auditory_amd.scan, on band_frames()).
+
 torch is used for what it is good at -- device memory, streams, torch.distributed (RCCL) --
 and never for arithmetic: every feature value comes out of libauditory_hip.so.
 """
@@ -91,6 +95,30 @@ class BatchProcessor:
         kwta_mod.kwta_batch_dev(params, gabor, act, pool=pool, state=state, cycles=cycles,
                                 device=self.plan.ctx.device, sum_order=sum_order, stream=self._stream())
         return act
+
+    def group_norm(self, maps, groups, weight=None, bias=None, eps=1e-5, act="relu", lengths=None, want_stats=False):
+        """Group norm with an activation on a feature map [n, PY, PX, ...channels] (the gabor output [n, PY, PX, 2, n_gabor]:
+        groups=2 is a group a polarity): every group of neighbouring channels is normalised over the item's positions, then
+        weight, bias [channels] and act.  Beside kwta() the other way from the raw maps to activations; for training use
+        auditory_amd.norm, which has the gradients."""
+        from . import norm
+        n, channels = maps.shape[0], maps[0, 0, 0].numel() if maps.dim() > 3 else maps.shape[-1]
+        flat = maps.reshape(n, -1, channels)
+        got = norm.group_norm(flat, groups, weight, bias, eps, act, lengths, want_stats=want_stats)
+        return (got[0].view(maps.shape), got[1]) if want_stats else got.view(maps.shape)
+
+    def process_norm(self, sig, items_dev, n_items, pools_y, pools_x, groups, weight=None, bias=None, eps=1e-5, act="relu"):
+        """ProcessSegment + ApplyGabor + group norm with an activation for every item, device-resident end to end:
+        returns (mel, raw gabor, normalised gabor)."""
+        mel, gab = self.process(sig, items_dev, n_items, pools_y, pools_x)
+        return mel, gab, self.group_norm(gab, groups, weight, bias, eps, act)
+
+    @staticmethod
+    def band_frames(maps):
+        """a feature map [n, PY, PX, ...channels] as sequences over time, one a band: [n * PY, PX, channels] (no copy) -- what
+        auditory_amd.scan's operators take"""
+        n, py, px = maps.shape[:3]
+        return maps.reshape(n * py, px, -1)
 
     def process_sndenv(self, sig, items_dev, n_items, pools_y, pools_x, params, state=None):
         """ProcessSegment + ApplyGabor with Kwta.On for every item, device-resident end to end:

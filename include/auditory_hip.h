@@ -496,7 +496,7 @@ int aud_kwta_batch_host(aud_ctx* ctx, const aud_kwta_params* k, const float* raw
  *  - lengths: int32 [n_items] in device memory, or NULL (every item is full).  Rows at and behind an item's length are
  *    padding: whatever they hold (NaN too) has no effect; outputs and gradients are written as zero there.  A value outside
  *    [0, rows] counts as the nearer end.
- *  - Results do not depend on other items of the batch, sums have a fixed order (no atomics): the same call gives the same bits.
+ *  - Sums have a fixed order (no atomics): the same call gives the same bits.
  *  - An output must not overlap an input, except state_out, which may be the state itself (same pointer).
  *  - workspace: device memory, 16-byte aligned, of the size that the _workspace_bytes function says for the SAME parameters;
  *    contents undefined before and after; NULL where that size is 0.  Calls on different streams, and captured graphs that may
@@ -508,7 +508,8 @@ int aud_kwta_batch_host(aud_ctx* ctx, const aud_kwta_params* k, const float* raw
 #define AUD_ACT_GELU 3 /* p (1 + erf(p / sqrt 2)) / 2; group norm only */
 
 /* group norm: x [n_items, rows, channels], `groups` groups of neighbouring channels, each normalised over rows x its channels
- * (the biased variance), then weight, bias and the activation.  1 <= channels <= 4096, a multiple of groups; eps > 0. */
+ * (the biased variance), then weight, bias and the activation.  1 <= channels <= 4096, a multiple of groups;
+ * eps > 0; at most 2^30 rows or steps in this and the following. */
 typedef struct {
     int32_t dtype, act, n_items, rows, channels, groups;
     float eps;

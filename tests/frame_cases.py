@@ -63,6 +63,18 @@ NORM = [
     (2, 64, 8, 2, "f32", "silu", True, None, 0, 1000.0),        # a level far from zero
     (3, 4, 12, 4, "f16", "gelu", False, "zero", 0, 0.0),        # nothing but padding
 ]
+# the routes that take larger sizes (on the GPU)
+NORM_BIG = [
+    (2, 600, 32, 4, "f32", "silu", True, "mixed", 0, 0.0),       # an item over several workgroups
+    (3, 777, 132, 12, "f16", "gelu", True, "mixed", 0, 0.0),     # packs of four
+    (1, 500, 33, 3, "bf16", "silu", True, None, 0, 0.0),         # one element at a time
+    (1, 100, 1024, 1024, "f32", "none", True, None, 0, 0.0),     # many groups: the chunks joined by a kernel of their own
+    (2, 40, 4096, 64, "bf16", "silu", True, "mixed", 0, 0.0),    # more packs than threads
+    (1, 9, 4095, 5, "f32", "relu", True, None, 0, 0.0),
+    (300, 5, 64, 4, "f32", "silu", True, "mixed", 0, 0.0),
+    (257, 300, 32, 8, "f32", "silu", True, None, 0, 0.0),        # an item in one workgroup, read twice
+    (2, 3000, 16, 2, "f32", "relu", True, None, 0, 300.0),
+]
 
 
 def norm_case(dev, items, rows, ch, groups, dtype, name, affine, lens, pad, level, seed=1):
@@ -129,6 +141,12 @@ CONV = [
     (5, 2, 16, 4, "f32", "none", True, True, "mixed", 5),        # shorter than the filter
     (2, 0, 8, 3, "f32", "silu", True, True, None, 0),            # no frame at all
 ]
+CONV_BIG = [
+    (3, 1030, 64, 4, "bf16", "silu", True, True, "mixed", 0),
+    (2, 517, 130, 3, "f16", "silu", True, True, None, 6),
+    (65, 1, 1024, 4, "f16", "silu", True, True, None, 0),
+    (1, 4100, 24, 2, "f32", "none", True, False, None, 0),
+]
 
 
 def conv_case(dev, items, steps, ch, taps, dtype, name, has_bias, has_state, lens, pad, seed=2):
@@ -182,6 +200,14 @@ SCAN = [
     (1, 130, 4, 1, 4, "f32", True, True, True, True, True, None, 0),     # a time axis cut into chunks
     (3, 200, 8, 1, 3, "bf16", True, False, True, True, True, "mixed", 0),
     (2, 0, 8, 1, 4, "f32", True, True, True, True, True, None, 0),       # no frame at all
+]
+SCAN_BIG = [
+    (1, 1000, 8, 1, 16, "f32", True, True, True, True, True, None, 0),      # more chunks than are folded
+    (170, 20, 8, 1, 4, "bf16", True, True, True, True, True, "mixed", 0),   # enough items: the axis is not cut
+    (2, 150, 200, 2, 64, "f16", True, True, True, True, True, "mixed", 0),  # four blocks of channels, 64 states
+    (2, 90, 65, 1, 24, "bf16", True, False, True, True, True, None, 3),     # odd blocks
+    (70, 1, 130, 1, 16, "bf16", True, True, True, True, True, None, 0),     # one frame
+    (450, 18, 8, 1, 8, "f32", True, True, True, True, False, "mixed", 0),   # gradients with an uncut axis
 ]
 
 
@@ -277,3 +303,89 @@ def scan_check(a, lengths, softplus, dy, ds, y, so, g):
     for n in names:
         assert (getattr(g, n) is None) == (a[n] is None), n
 
+
+
+# ---- one frame at a time against the whole ---------------------------------------------------------------------------------
+
+def stream_case(dev, items, steps, ch, groups, states, dtype, seed=5):
+    """frames one by one, with the states carried in place, against one call: the convolution bit for bit, the scan within the
+    bounds of both"""
+    m = Make(dev, seed, dtype)
+    x = m.n(items, steps, ch)
+    w, b = m.n(ch, 4, f32=True, scale=0.5), m.n(ch, f32=True, scale=0.2)
+    s0 = m.n(items, 3, ch)
+    s = s0.clone()
+    whole = scan.causal_conv(x, w, b, act="silu", state=s0)
+    parts = torch.stack([scan.causal_conv_step(x[:, t], s, w, b, act="silu") for t in range(steps)], 1)
+    assert torch.equal(whole, parts)
+    assert torch.equal(s, torch.cat([s0, x], 1)[:, -3:])
+    a = scan_inputs(m, items, steps, ch, groups, states, True, True, True, True, True)
+    h = a["state"].clone()
+    ys = []
+    for t in range(steps):
+        ys.append(scan.selective_scan_step(a["u"][:, t], a["delta"][:, t], a["A"], a["B"][:, t], a["C"][:, t], h, D=a["D"],
+                                           z=a["z"][:, t], delta_bias=a["delta_bias"], softplus=True))
+    scan_check(a, None, True, a["u"], torch.zeros_like(h), torch.stack(ys, 1), h, None)
+
+
+# ---- gradients against differences -----------------------------------------------------------------------------------------
+
+def difference(name, value, exact, point, grad, direction, h):
+    """The directional derivative by central differences.  `value` (the kernels, float32) and `exact` (64 bits) are the loss at
+    a point; their differences at the same h have the same truncation, so they may differ by rounding alone: each loss is good
+    to r = |loss terms| k u, divided by h.  The gradient is held to the exact difference, whose truncation is 4/3 of what halving
+    h changes."""
+    up = [p + h * d for p, d in zip(point, direction)]
+    down = [p - h * d for p, d in zip(point, direction)]
+    (lu, mu), (ld, _) = value(up), value(down)
+    got = (lu - ld) / (2 * h)
+
+    def central(step):
+        f = [exact([p.double() + s * step * d.double() for p, d in zip(point, direction)]) for s in (1, -1)]
+        return (f[0] - f[1]) / (2 * step)
+
+    ref, half = central(h), central(h / 2)
+    rounding = mu * 400 * R.U / h
+    assert abs(got - ref) <= rounding, (name, got, ref, rounding)
+    along = sum(float((g.double() * d.double()).sum()) for g, d in zip(grad, direction))
+    truncation = abs(ref - half) * 4 / 3
+    assert abs(along - ref) <= 2 * truncation + rounding, (name, along, ref, truncation, rounding)
+
+
+def difference_cases(dev):
+    m = Make(dev, 11, "f32")
+    x, w, b, dy = m.n(2, 7, 12), m.n(12, f32=True), m.n(12, f32=True), m.n(2, 7, 12)
+    c64 = dy.cpu().double()
+    y, st = norm.group_norm(x, 3, w, b, act="silu", want_stats=True)
+    g = norm.group_norm_grad(dy, x, st, 3, w, b, act="silu")
+
+    def loss(y):
+        t = (y.cpu().double() * c64)
+        return float(t.sum()), float(t.abs().sum())
+
+    difference("norm", lambda p: loss(norm.group_norm(p[0], 3, p[1], p[2], act="silu")),
+               lambda p: float((R.norm(p[0].cpu(), 3, p[1].cpu(), p[2].cpu(), 1e-5, "silu", None)[0] * c64).sum()),
+               [x, w, b], g, [m.n(2, 7, 12), m.n(12), m.n(12)], 2.0 ** -6)
+    cw, cb, s = m.n(12, 3), m.n(12), m.n(2, 2, 12)
+    g = scan.causal_conv_grad(dy, x, cw, cb, act="silu", state=s)
+    difference("conv", lambda p: loss(scan.causal_conv(p[0], p[1], p[2], act="silu", state=p[3])),
+               lambda p: float((R.conv(*[t.cpu() for t in p[:3]], "silu", p[3].cpu(), None)[0] * c64).sum()),
+               [x, cw, cb, s], g, [m.n(2, 7, 12), m.n(12, 3), m.n(12), m.n(2, 2, 12)], 2.0 ** -6)
+    a = scan_inputs(m, 2, 7, 12, 2, 4, True, True, True, True, True)
+    names = ("u", "delta", "A", "B", "C", "D", "z", "delta_bias", "state")
+
+    def run(p, keep=False):
+        q = dict(zip(names, p))
+        return scan.selective_scan(q["u"], q["delta"], q["A"], q["B"], q["C"], D=q["D"], z=q["z"], delta_bias=q["delta_bias"],
+                                   softplus=True, state=q["state"], keep=keep)
+
+    def ref(p):
+        q = dict(zip(names, [t.cpu() for t in p]))
+        return float((R.scan(q["u"], q["delta"], q["A"], q["B"], q["C"], q["D"], q["z"], q["delta_bias"], True, q["state"], None)[0]
+                      * c64).sum())
+
+    point = [a[n] for n in names]
+    _, kept = run(point, True)
+    g = scan.selective_scan_grad(dy, a["u"], a["delta"], a["A"], a["B"], a["C"], kept, D=a["D"], z=a["z"],
+                                 delta_bias=a["delta_bias"], softplus=True, state=a["state"])
+    difference("scan", lambda p: loss(run(p)), ref, point, g, [m.n(*t.shape) for t in point], 2.0 ** -7)
