@@ -80,6 +80,28 @@ def _build(force, verbose, objdir, LIB, extra):
     return LIB
 
 
+TORCH_SRC = os.path.join(CSRC, "frames_torch.cpp")
+TORCH_LIB = os.path.join(HERE, "_frames.so")
+
+
+def build_torch(force=False):
+    """auditory_amd/_frames.so: the torch side of the operators in norm.py and scan.py (host code only, g++).  It is loaded by
+    Python and calls libauditory_hip.so through addresses, so it links torch alone."""
+    deps = [TORCH_SRC, os.path.join(INCLUDE, "auditory_hip.h")]
+    if not force and os.path.exists(TORCH_LIB) and all(os.path.getmtime(d) <= os.path.getmtime(TORCH_LIB) for d in deps):
+        return TORCH_LIB
+    import sysconfig
+    import torch
+    t = os.path.dirname(torch.__file__)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    subprocess.check_call(
+        ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_API_INCLUDE_EXTENSION_H",
+         "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI), "-I" + INCLUDE, "-isystem", t + "/include",
+         "-isystem", t + "/include/torch/csrc/api/include", "-isystem", sysconfig.get_paths()["include"], "-isystem", rocm + "/include",
+         TORCH_SRC, "-o", TORCH_LIB, "-L" + t + "/lib", "-Wl,-rpath," + t + "/lib", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
+    return TORCH_LIB
+
+
 UBENCH_SRC = os.path.join(os.path.dirname(HERE), "tools", "ubench", "stream_read.hip")
 UBENCH_LIB = os.path.join(os.path.dirname(HERE), "tools", "ubench", "libstream_read.so")
 
@@ -102,3 +124,4 @@ if __name__ == "__main__":
         print(build(tag=t, defines=[a for a in argv if a.startswith("-D")] + extra, verbose=True))
     else:
         print(build(force=True, verbose=True))
+        print(build_torch(force=True))

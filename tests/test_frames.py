@@ -30,11 +30,11 @@ def emu_lib():
 @pytest.fixture
 def emu(emu_lib, monkeypatch):
     """the operators on CPU tensors, their kernels run by the thread emulator"""
-    monkeypatch.setattr(frames, "context", lambda x, name: runtime.get_ctx(0))
-    monkeypatch.setattr(frames, "current_stream", lambda index: None)
+    native = frames.native()
+    monkeypatch.setattr(frames, "context", lambda x, name: runtime.get_ctx(0).handle.value)
+    frames.bind(native, emu_lib, False)
     yield emu_lib
-    for plans in (norm._PLANS, scan._CONV_PLANS, scan._SCAN_PLANS):  # (they hold the emulator's context)
-        plans.clear()
+    frames.bind(native, C.CDLL(capi.LIB_PATH), True)
 
 
 # ---- values and gradients ------------------------------------------------------------------------------------------------
