@@ -44,6 +44,12 @@ struct Input {
         return reinterpret_cast<uintptr_t>(p) % bytes == 0 && (rows <= 1 || row * e % bytes == 0) && (items <= 1 || item * e % bytes == 0);
     }
 };
+template <typename F>
+int alignment(int e, F&& fits) {  // the largest of 16, 8, 4 (and e) bytes that fits() says everything is a multiple of
+    for (int b = 16; b > e; b /= 2)
+        if (fits(b)) return b;
+    return e;
+}
 bool at(const void* p, int bytes) { return !p || reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
@@ -187,7 +193,7 @@ int aud_group_norm_batch_dev(aud_ctx* c, const aud_norm_params* p, const void* x
     const Range outs[] = {{y, n * e}, {stats, st}, {workspace, need}};
     const Range ins[] = {{x, in.span(e)}, {weight, ch}, {bias, ch}, {lengths, 4 * int64_t(p->n_items)}};
     if (clash(outs, 3, ins, 4)) return fail(c, AUD_EINVAL, "an output overlaps another buffer");
-    const int align = in.aligned(16, e) && at(y, 16) ? 16 : in.aligned(8, e) && at(y, 8) ? 8 : e;
+    const int align = alignment(e, [&](int b) { return in.aligned(b, e) && at(y, b); });
     const aud::NormRoute r = norm_route_of(p, align, false);
     if (int64_t(p->n_items) * r.chunks > kMaxGrid - 64 || int64_t(p->n_items) * (p->channels / 32 + 1) > kMaxGrid) return fail(c, AUD_EINVAL, "too many items");
     const OnDevice device(c);
@@ -230,7 +236,7 @@ int aud_group_norm_grad_dev(aud_ctx* c, const aud_norm_params* p, const void* dy
             AUD_HIP(c, aud::launch_column_sums(nullptr, 0, p->channels, 0, 2, nullptr, dweight, dbias, static_cast<hipStream_t>(stream)));
         return AUD_OK;
     }
-    const int align = in.aligned(16, e) && g.aligned(16, e) && at(dx, 16) ? 16 : in.aligned(8, e) && g.aligned(8, e) && at(dx, 8) ? 8 : e;
+    const int align = alignment(e, [&](int b) { return in.aligned(b, e) && g.aligned(b, e) && at(dx, b); });
     const aud::NormRoute r = norm_route_of(p, align, true);
     if (int64_t(p->n_items) * r.chunks > kMaxGrid - 64 || int64_t(p->n_items) * (p->channels / 32 + 1) > kMaxGrid) return fail(c, AUD_EINVAL, "too many items");
     aud::NormArgs a{};
@@ -261,24 +267,24 @@ int aud_causal_conv_batch_dev(aud_ctx* c, const aud_conv_params* p, const void* 
     const Range ins[] = {{x, in.span(e)}, {weight, ch * p->taps}, {bias, ch}, {lengths, 4 * int64_t(p->n_items)},
                          {state == state_out ? nullptr : state, ns * e}};
     if (clash(outs, 2, ins, 5)) return fail(c, AUD_EINVAL, "an output overlaps another buffer");
-    const bool aligned = in.aligned(16, e) && at(y, 16) && at(state, 16) && at(state_out, 16);
+    const int align = alignment(e, [&](int b) { return in.aligned(b, e) && at(y, b) && at(state, b) && at(state_out, b); });
     aud::ConvArgs a{};
-    a.T = aud::conv_tile(p->dtype, p->n_items, p->steps, p->channels, aligned, false);
+    a.T = aud::conv_tile(p->dtype, p->n_items, p->steps, p->channels, align);
     if (int64_t(p->n_items) * conv_tiles(p, a.T) > kMaxGrid * 64 / p->channels) return fail(c, AUD_EINVAL, "tensor too large for one call");
     const OnDevice device(c);
     AUD_HIP(c, device.err);
     a.x = x, a.weight = weight, a.bias = bias, a.state = state, a.lengths = lengths, a.out = y, a.state_out = state_out;
     a.B = p->n_items, a.L = p->steps, a.D = p->channels, a.xi = p->x_item, a.xr = p->x_row;
-    AUD_HIP(c, aud::launch_conv(a, p->dtype, p->act, p->taps, aligned, static_cast<hipStream_t>(stream)));
+    AUD_HIP(c, aud::launch_conv(a, p->dtype, p->act, p->taps, align, static_cast<hipStream_t>(stream)));
     return AUD_OK;
 }
 
 int aud_causal_conv_workspace_bytes(const aud_conv_params* p, int64_t* bytes) {
     if (!bytes || conv_bad(p, true)) return AUD_EINVAL;
-    // the larger of the two routes' (aligned or not)
+    // the largest of the routes' (by alignment)
     int64_t tiles = 0;
-    for (int aligned = 0; aligned < 2; ++aligned)
-        tiles = std::max(tiles, conv_tiles(p, aud::conv_tile(p->dtype, p->n_items, p->steps, p->channels, aligned != 0, true)));
+    for (int align = 2; align <= 16; align *= 2)
+        tiles = std::max(tiles, conv_tiles(p, aud::conv_tile(p->dtype, p->n_items, p->steps, p->channels, align)));
     *bytes = 4 * int64_t(p->n_items) * tiles * (p->taps + 1) * p->channels;
     return AUD_OK;
 }
@@ -310,15 +316,16 @@ int aud_causal_conv_grad_dev(aud_ctx* c, const aud_conv_params* p, const void* d
             AUD_HIP(c, aud::launch_column_sums(nullptr, 0, p->channels, p->taps, 1, dweight, dbias, nullptr, static_cast<hipStream_t>(stream)));
         return AUD_OK;
     }
-    const bool aligned = in.aligned(16, e) && g.aligned(16, e) && at(dx, 16) && at(state, 16) && at(dstate_out, 16) && at(dstate, 16);
+    const int align = alignment(
+        e, [&](int b) { return in.aligned(b, e) && g.aligned(b, e) && at(dx, b) && at(state, b) && at(dstate_out, b) && at(dstate, b); });
     aud::ConvArgs a{};
-    a.T = aud::conv_tile(p->dtype, p->n_items, p->steps, p->channels, aligned, true);
+    a.T = aud::conv_tile(p->dtype, p->n_items, p->steps, p->channels, align);
     if (int64_t(p->n_items) * conv_tiles(p, a.T) > kMaxGrid * 64 / p->channels) return fail(c, AUD_EINVAL, "tensor too large for one call");
     a.x = x, a.dy = dy, a.weight = weight, a.bias = bias, a.state = state, a.lengths = lengths, a.out = dx;
     a.dstate_out = dstate_out, a.dstate = dstate, a.dweight = dweight, a.dbias = dbias, a.part = static_cast<float*>(workspace);
     a.B = p->n_items, a.L = p->steps, a.D = p->channels;
     a.xi = p->x_item, a.xr = p->x_row, a.di = p->dy_item, a.dr = p->dy_row;
-    AUD_HIP(c, aud::launch_conv_grad(a, p->dtype, p->act, p->taps, aligned, static_cast<hipStream_t>(stream)));
+    AUD_HIP(c, aud::launch_conv_grad(a, p->dtype, p->act, p->taps, align, static_cast<hipStream_t>(stream)));
     return AUD_OK;
 }
 

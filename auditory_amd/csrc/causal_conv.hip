@@ -240,32 +240,39 @@ hipError_t by_taps(const ConvArgs& a, int act, int K, bool grad, hipStream_t st)
         default: return hipErrorInvalidValue;
     }
 }
-hipError_t by_type(const ConvArgs& a, int dtype, int act, int K, bool aligned, bool grad, hipStream_t st) {
-    const int e = dtype == AUD_F32 ? 4 : 2;
-    const bool vec = aligned && a.D % (16 / e) == 0;
+hipError_t by_type(const ConvArgs& a, int dtype, int act, int K, int align, bool grad, hipStream_t st) {
+    const int v = vector_of(dtype == AUD_F32 ? 4 : 2, a.D, align);
     switch (dtype) {
-        case AUD_F32: return vec ? by_taps<AUD_F32, 4>(a, act, K, grad, st) : by_taps<AUD_F32, 1>(a, act, K, grad, st);
-        case AUD_BF16: return vec ? by_taps<AUD_BF16, 8>(a, act, K, grad, st) : by_taps<AUD_BF16, 1>(a, act, K, grad, st);
-        default: return vec ? by_taps<AUD_F16, 8>(a, act, K, grad, st) : by_taps<AUD_F16, 1>(a, act, K, grad, st);
+        case AUD_F32:
+            return v == 4   ? by_taps<AUD_F32, 4>(a, act, K, grad, st)
+                   : v == 2 ? by_taps<AUD_F32, 2>(a, act, K, grad, st)
+                            : by_taps<AUD_F32, 1>(a, act, K, grad, st);
+        case AUD_BF16:
+            return v == 8   ? by_taps<AUD_BF16, 8>(a, act, K, grad, st)
+                   : v >= 2 ? by_taps<AUD_BF16, 2>(a, act, K, grad, st)
+                            : by_taps<AUD_BF16, 1>(a, act, K, grad, st);
+        default:
+            return v == 8   ? by_taps<AUD_F16, 8>(a, act, K, grad, st)
+                   : v >= 2 ? by_taps<AUD_F16, 2>(a, act, K, grad, st)
+                            : by_taps<AUD_F16, 1>(a, act, K, grad, st);
     }
 }
 
 }  // namespace
 
 // steps a thread walks: as many as leave the card about 2048 waves, between 8 and 64
-int conv_tile(int dtype, int B, int L, int D, bool aligned, bool) {
-    const int e = dtype == AUD_F32 ? 4 : 2;
-    const int V = aligned && D % (16 / e) == 0 ? 16 / e : 1;
+int conv_tile(int dtype, int B, int L, int D, int align) {
+    const int v = vector_of(dtype == AUD_F32 ? 4 : 2, D, align), V = dtype != AUD_F32 && v == 4 ? 2 : v;
     int T = 64;
     while (T > 8 && int64_t(B) * (D / V) * ((L + T - 1) / T) < 64 * 2048) T /= 2;
     return T;
 }
 
-hipError_t launch_conv(const ConvArgs& a, int dtype, int act, int K, bool aligned, hipStream_t st) {
-    return by_type(a, dtype, act, K, aligned, false, st);
+hipError_t launch_conv(const ConvArgs& a, int dtype, int act, int K, int align, hipStream_t st) {
+    return by_type(a, dtype, act, K, align, false, st);
 }
-hipError_t launch_conv_grad(const ConvArgs& a, int dtype, int act, int K, bool aligned, hipStream_t st) {
-    return by_type(a, dtype, act, K, aligned, true, st);
+hipError_t launch_conv_grad(const ConvArgs& a, int dtype, int act, int K, int align, hipStream_t st) {
+    return by_type(a, dtype, act, K, align, true, st);
 }
 
 }  // namespace aud

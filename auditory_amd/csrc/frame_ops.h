@@ -71,8 +71,8 @@ __device__ __forceinline__ float fast_sigmoid(float x) { return __builtin_amdgcn
 __device__ __forceinline__ float softplus(float x) {
     const float e = __builtin_amdgcn_exp2f(-kLog2e * fabsf(x));
     const float w = 1.f + e, d = w - 1.f;
-    const float l = kLn2 * __builtin_amdgcn_logf(w);
-    return fmaxf(x, 0.f) + (d == 0.f ? e : l * (e * __builtin_amdgcn_rcpf(d)));
+    const float l = kLn2 * __builtin_amdgcn_logf(w) * (e * __builtin_amdgcn_rcpf(fmaxf(d, 1e-30f)));
+    return fmaxf(x, 0.f) + (d > 0.f ? l : e);
 }
 template <int ACT>
 __device__ __forceinline__ float act_value(float p) {
@@ -98,6 +98,9 @@ __device__ __forceinline__ int item_rows(const int32_t* lengths, int b, int rows
     const int n = lengths[b];
     return n < 0 ? 0 : (n > rows ? rows : n);
 }
+
+// elements per access for rows of C elements of e bytes, where all addresses and strides are multiples of `align` bytes
+int vector_of(int e, int C, int align);
 
 // ---- launch descriptors ----------------------------------------------------------------------------------------------
 struct NormArgs {
@@ -141,9 +144,9 @@ struct ConvArgs {
     int64_t xi, xr, di, dr;
     int T;                    // steps a thread walks
 };
-int conv_tile(int dtype, int B, int L, int D, bool aligned, bool grad);
-hipError_t launch_conv(const ConvArgs& a, int dtype, int act, int K, bool aligned, hipStream_t st);
-hipError_t launch_conv_grad(const ConvArgs& a, int dtype, int act, int K, bool aligned, hipStream_t st);
+int conv_tile(int dtype, int B, int L, int D, int align);
+hipError_t launch_conv(const ConvArgs& a, int dtype, int act, int K, int align, hipStream_t st);
+hipError_t launch_conv_grad(const ConvArgs& a, int dtype, int act, int K, int align, hipStream_t st);
 
 constexpr int kScanTile = 16;  // steps between kept states; the kernels' unit of work along the time axis
 struct ScanArgs {

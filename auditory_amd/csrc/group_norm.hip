@@ -649,14 +649,18 @@ hipError_t by_act(const NormArgs& a, const NormRoute& r, int act, bool grad, hip
 hipError_t by_type(const NormArgs& a, const NormRoute& r, int dtype, int act, bool grad, hipStream_t st) {
     switch (dtype) {
         case AUD_F32:
-            return r.vec == 4 ? by_act<AUD_F32, 4>(a, r, act, grad, st) : by_act<AUD_F32, 1>(a, r, act, grad, st);
+            return r.vec == 4   ? by_act<AUD_F32, 4>(a, r, act, grad, st)
+                   : r.vec == 2 ? by_act<AUD_F32, 2>(a, r, act, grad, st)
+                                : by_act<AUD_F32, 1>(a, r, act, grad, st);
         case AUD_BF16:
             return r.vec == 8   ? by_act<AUD_BF16, 8>(a, r, act, grad, st)
                    : r.vec == 4 ? by_act<AUD_BF16, 4>(a, r, act, grad, st)
+                   : r.vec == 2 ? by_act<AUD_BF16, 2>(a, r, act, grad, st)
                                 : by_act<AUD_BF16, 1>(a, r, act, grad, st);
         default:
             return r.vec == 8   ? by_act<AUD_F16, 8>(a, r, act, grad, st)
                    : r.vec == 4 ? by_act<AUD_F16, 4>(a, r, act, grad, st)
+                   : r.vec == 2 ? by_act<AUD_F16, 2>(a, r, act, grad, st)
                                 : by_act<AUD_F16, 1>(a, r, act, grad, st);
     }
 }
@@ -670,10 +674,16 @@ hipError_t launch_column_sums(const float* in, int64_t rows, int W, int K, int e
     return hipGetLastError();
 }
 
+int vector_of(int e, int C, int align) {
+    for (int v = 16 / e; v > 1; v /= 2)
+        if (align >= v * e && C % v == 0) return v;
+    return 1;
+}
+
 NormRoute norm_route(int dtype, int B, int S, int C, int G, int align, bool) {
     NormRoute r{};
     const int e = dtype == AUD_F32 ? 4 : 2;
-    r.vec = align >= 16 && C % (16 / e) == 0 ? 16 / e : align >= 8 && e == 2 && C % 4 == 0 ? 4 : 1;
+    r.vec = vector_of(e, C, align);
     const int64_t bytes = int64_t(S) * C * e;
     r.one_wg = bytes <= 32 * 1024 || (B >= 256 && bytes <= 128 * 1024) || (B >= 1024 && bytes <= 1024 * 1024);
     r.chunks = 1;

@@ -147,6 +147,13 @@ __device__ __forceinline__ void store_some(void* base, int64_t at, int c, int dn
 }
 
 __device__ __forceinline__ float step_size(float raw, int softp) { return softp ? softplus(raw) : raw; }
+// (one branch for all of a thread's elements, so that their chains run side by side)
+template <int E>
+__device__ __forceinline__ void step_sizes(float (&dt)[E], int softp) {
+    if (softp)
+#pragma unroll
+        for (int i = 0; i < E; ++i) dt[i] = softplus(dt[i]);
+}
 
 // B and C in float32 -> table [B, G, tiles, waves, 16 steps, B or C, NW states]: what a wave reads of a tile is one run.  States
 // past N and steps at and behind the item's length are 0.
@@ -266,15 +273,20 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     raw* py = PASS == 3 ? static_cast<raw*>(a.y) + y0 + int64_t(first * kT + pt) * a.Dn : nullptr;
     float u[E], z[E];  // of the tile that is being scanned
     auto stage = [&](int tile, int buf) {
-        float step[2 * E];
+        float step[2 * E], dt[E];
+        const bool row_on = tile * kT + pt < len;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const bool on = tile * kT + pt < len && c + i < at.dn;
+            const bool on = row_on && c + i < at.dn;
             u[i] = on ? ru.get(i) : 0.f;
             z[i] = on ? rz.get(i) : 0.f;
-            const float dt = on ? step_size(rd.get(i) + bias[i], a.softplus) : 0.f;
-            step[2 * i] = dt;
-            step[2 * i + 1] = dt * u[i];
+            dt[i] = rd.get(i) + bias[i];
+        }
+        step_sizes(dt, a.softplus);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            step[2 * i] = row_on && c + i < at.dn ? dt[i] : 0.f;
+            step[2 * i + 1] = step[2 * i] * u[i];
         }
         lds_write(lds + 2 * ((buf * kT + pt) * kCh + c), step);
     };
@@ -340,11 +352,11 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
 #pragma unroll
                 for (int i = 0; i < E; ++i) y[i] += part[i];
             }
+            if (a.z)
 #pragma unroll
-            for (int i = 0; i < E; ++i) {
-                if (a.z) y[i] *= sz[i] * fast_sigmoid(sz[i]);
-                if (t >= len) y[i] = 0.f;
-            }
+                for (int i = 0; i < E; ++i) y[i] *= sz[i] * fast_sigmoid(sz[i]);
+#pragma unroll
+            for (int i = 0; i < E; ++i) y[i] = t < len ? y[i] : 0.f;
             store_some<DT, E, VEC>(py, 0, c, at.dn, y);
         }
         if (PASS == 3) py += kT * a.Dn;
@@ -510,11 +522,11 @@ struct LaneSums {
     static __device__ __forceinline__ bool first_of(int lane) { return (lane & ((1 << (6 - USED)) - 1)) == 0; }
 };
 
-// PASS 1: what a chunk hands to the one in front of it, from a zero carry, and its sum of dt; PASS 3: everything.  Four waves
-// of NW states each.
-template <int DT, int NW, bool VEC, int PASS>
-__global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
-    constexpr int W = 4, NP = W * NW, E = 4, ROW = kCh / E;
+// PASS 1: what a chunk hands to the one in front of it, from a zero carry, and its sum of dt; PASS 3: everything.  W waves of NW
+// states each.
+template <int DT, int NW, int W, bool VEC, int PASS>
+__global__ void __launch_bounds__(64 * W, 2) k_scan_grad(ScanArgs a, int blocks) {
+    constexpr int NP = W * NW, E = 16 / W, ROW = kCh / E;
     constexpr int TS = NW <= 4 ? 16 : 64 / NW, SUBS = kT / TS;  // steps whose states are in registers at once
     float* lds = reinterpret_cast<float*>(dyn_lds());
     float* s_dt = lds;                      // [16][64] each
@@ -522,7 +534,7 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
     float* s_du = s_f + kT * kCh;           // dt u
     float* s_db = s_du + kT * kCh;          // [16][NP] each
     float* s_dc = s_db + kT * NP;
-    float* s_sum = s_dc + kT * NP;          // [3][4][16][64]: sum_n g B, sum_n A a h g, sum_n C h of each wave
+    float* s_sum = s_dc + kT * NP;          // [3][W][16][64]: sum_n g B, sum_n A a h g, sum_n C h of each wave
     const Where at(a, blocks, 0, PASS == 1);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int pt = tid / ROW, c = (tid % ROW) * E;
@@ -542,12 +554,13 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
         if (there && at.chunk == a.chunks - 1 && a.dstate_out) carry[i] = a.dstate_out[(int64_t(at.b) * a.Dn + d) * a.N + n];
     }
     if (PASS == 3 && at.chunk < a.chunks - 1) chunk_state<NW, true>(a, at, wave * NW, d, live, A2, carry);
-    float skip[E], bias[E], sum_fu[E] = {0.f, 0.f, 0.f, 0.f}, sum_dd[E] = {0.f, 0.f, 0.f, 0.f};
+    float skip[E], bias[E], sum_fu[E], sum_dd[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
         const bool there = c + i < at.dn;
         skip[i] = there && a.D ? a.D[at.d0 + c + i] : 0.f;
         bias[i] = there && a.delta_bias ? a.delta_bias[at.d0 + c + i] : 0.f;
+        sum_fu[i] = sum_dd[i] = 0.f;
     }
     const int first = at.chunk * a.chunk_tiles, end = first + a.chunk_tiles < tiles ? first + a.chunk_tiles : tiles;
     Raw<DT, E, VEC> ru{}, rd{}, rz{}, ry{};
@@ -581,8 +594,16 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
             z[i] = there ? rz.get(i) : 0.f;
             dy[i] = there ? ry.get(i) : 0.f;
             arg[i] = (there ? rd.get(i) : 0.f) + bias[i];
-            dt[i] = there ? step_size(arg[i], a.softplus) : 0.f;
-            f[i] = a.z ? dy[i] * (z[i] * fast_sigmoid(z[i])) : dy[i];
+            dt[i] = arg[i];
+            f[i] = dy[i];
+        }
+        step_sizes(dt, a.softplus);
+        if (a.z)
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] *= z[i] * fast_sigmoid(z[i]);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            if (!(on && c + i < at.dn)) dt[i] = 0.f;
             dtu[i] = dt[i] * u[i];
         }
         lds_write(s_dt + pt * kCh + c, dt);
@@ -621,16 +642,27 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
                 float h[NW], hs[TS][NW], as[TS][NW];  // states behind and decays of the steps of this part of the tile
 #pragma unroll
                 for (int i = 0; i < NW; ++i) h[i] = hs0[i];
-                if constexpr (SUBS > 1)
-                    for (int k = 0; k < k0; ++k)
+                Vec next;
+                next.template load<true, true>(bc);
+                if constexpr (SUBS > 1) {  // up to this part: once more from the tile's first state
+#pragma unroll 1
+                    for (int q = 0; q < k0; q += GS) {
+                        const Vec now = next;
+                        float s[GS], x[GS];
 #pragma unroll
-                        for (int i = 0; i < NW; ++i)
-                            h[i] = fmaf(exp2_hw(s_dt[k * kCh + lane] * A2[i]), h[i], s_du[k * kCh + lane] * bc[k * 2 * NW + i]);
+                        for (int k = 0; k < GS; ++k) s[k] = s_dt[(q + k) * kCh + lane], x[k] = s_du[(q + k) * kCh + lane];
+                        wait_lds();
+                        next.template load<true, true>(bc + (q + GS) * 2 * NW);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int k = 0; k < GS; ++k)
+#pragma unroll
+                            for (int i = 0; i < NW; ++i) h[i] = fmaf(exp2_hw(s[k] * A2[i]), h[i], x[k] * now.b[k][i]);
+                    }
+                }
                 float before[NW];
 #pragma unroll
                 for (int i = 0; i < NW; ++i) before[i] = h[i];
-                Vec next;
-                next.template load<true, true>(bc + k0 * 2 * NW);
 #pragma unroll
                 for (int q = 0; q < TS; q += GS) {
                     const Vec now = next;
@@ -718,12 +750,22 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
                 for (int i = 0; i < E; ++i) {
                     const float ddt = fmaf(u[i], sums[0][i], sums[1][i]);
                     du[i] = fmaf(dt[i], sums[0][i], skip[i] * f[i]);
-                    dd[i] = on ? ddt * (a.softplus ? fast_sigmoid(arg[i]) : 1.f) : 0.f;
-                    const float q = fast_sigmoid(z[i]);
-                    dz[i] = dy[i] * fmaf(skip[i], u[i], sums[2][i]) * (q * (1.f + z[i] * (1.f - q)));
+                    dd[i] = ddt;
                     sum_fu[i] = fmaf(f[i], u[i], sum_fu[i]);
+                }
+                if (a.softplus)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) dd[i] *= fast_sigmoid(arg[i]);
+                if (a.z)
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const float q = fast_sigmoid(z[i]);
+                        dz[i] = dy[i] * fmaf(skip[i], u[i], sums[2][i]) * (q * (1.f + z[i] * (1.f - q)));
+                    }
+#pragma unroll
+                for (int i = 0; i < E; ++i) {
+                    if (!on) du[i] = dd[i] = dz[i] = 0.f;
                     sum_dd[i] += dd[i];
-                    if (!on) du[i] = dz[i] = 0.f;
                 }
                 const int64_t o = o0 + int64_t(t) * a.Dn;
                 store_some<DT, E, VEC>(a.du, o, c, at.dn, du);
@@ -732,7 +774,7 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
             }
             // dB, dC of the tile, summed over this block's channels: partial sums where the group has more blocks
             const int64_t table = int64_t(a.B) * a.L * a.G * a.N;
-            for (int i = tid; i < kT * NP; i += kNT) {
+            for (int i = tid; i < kT * NP; i += 64 * W) {
                 const int k = i / NP, n = i % NP;
                 if (n >= a.N || t0 + k >= a.L) continue;
                 const int64_t o = ((int64_t(at.b) * a.L + t0 + k) * a.G + at.g) * a.N + n;
@@ -756,13 +798,13 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
             if (wave * NW + i < a.N) a.sums[((int64_t(at.b) * a.chunks + at.chunk) * a.N + wave * NW + i) * a.Dn + d] = carry[i];
         if (wave == 0) dt_sums[(int64_t(at.b) * a.chunks + at.chunk) * a.Dn + d] = sum_dt;
     } else {
-        float* row = a.part + (int64_t(at.b) * a.chunks + at.chunk) * (a.N + 2) * a.Dn;
+        float* sums_of = a.part + (int64_t(at.b) * a.chunks + at.chunk) * (a.N + 2) * a.Dn;
         if (live) {
 #pragma unroll
             for (int i = 0; i < NW; ++i) {
                 const int n = wave * NW + i;
                 if (n >= a.N) continue;
-                row[int64_t(n) * a.Dn + d] = dA[i];
+                sums_of[int64_t(n) * a.Dn + d] = dA[i];
                 if (at.chunk == 0 && a.dstate) a.dstate[(int64_t(at.b) * a.Dn + d) * a.N + n] = carry[i];
             }
         }
@@ -776,7 +818,7 @@ __global__ void __launch_bounds__(kNT, 2) k_scan_grad(ScanArgs a, int blocks) {
             const float* p = (wave == 0 ? s_dt : s_f) + lane;
             float s = 0.f;
             for (int k = 0; k < kT; ++k) s += p[k * kCh];
-            row[int64_t(a.N + wave) * a.Dn + d] = s;
+            sums_of[int64_t(a.N + wave) * a.Dn + d] = s;
         }
     }
 }
@@ -822,22 +864,22 @@ hipError_t run(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 3>), grid, wg, lds3, st, a, r.blocks);
     return hipGetLastError();
 }
-template <int DT, int NW, bool VEC>
+template <int DT, int NW, int W, bool VEC>
 hipError_t run_grad(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
-    constexpr int NP = 4 * NW;
+    constexpr int NP = W * NW;
     const dim3 grid(unsigned(int64_t(a.B) * a.chunks * a.G * r.blocks));
-    const size_t lds1 = size_t(2) * kT * kCh * 4, lds3 = size_t(3 * kT * kCh + 2 * kT * NP + 12 * kT * kCh) * 4;
-    if (hipError_t e = allow_lds(&k_scan_grad<DT, NW, VEC, 3>, lds3)) return e;
+    const size_t lds1 = size_t(2) * kT * kCh * 4, lds3 = size_t(3 * kT * kCh + 2 * kT * NP + 3 * W * kT * kCh) * 4;
+    if (hipError_t e = allow_lds(&k_scan_grad<DT, NW, W, VEC, 3>, lds3)) return e;
     run_table<DT>(a, NP, NW, st);
     if (a.chunks > 1) {
         const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 1>), first, dim3(kNT), lds1, st, a, r.blocks);
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, W, VEC, 1>), first, dim3(64 * W), lds1, st, a, r.blocks);
         if (a.chunks > kFoldChunks) {
             const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
             hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<true>), dim3(join), dim3(kJoinThreads), 0, st, a);
         }
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, VEC, 3>), grid, dim3(kNT), lds3, st, a, r.blocks);
+    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, W, VEC, 3>), grid, dim3(64 * W), lds3, st, a, r.blocks);
     const int64_t bc = 2 * int64_t(a.B) * a.L * a.G * a.N;
     if (bc > 0 && r.blocks > 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_bc<DT>), dim3(unsigned((bc + kNT - 1) / kNT)), dim3(kNT), 0, st, a, r.blocks);
     if (hipError_t e = hipGetLastError()) return e;
@@ -848,11 +890,11 @@ hipError_t by_states(const ScanArgs& a, const ScanRoute& r, bool grad, hipStream
     const int NP = scan_padded_states(a.N);
     if (grad) {
         switch (NP) {
-            case 4: return run_grad<DT, 1, VEC>(a, r, st);
-            case 8: return run_grad<DT, 2, VEC>(a, r, st);
-            case 16: return run_grad<DT, 4, VEC>(a, r, st);
-            case 32: return run_grad<DT, 8, VEC>(a, r, st);
-            default: return run_grad<DT, 16, VEC>(a, r, st);
+            case 4: return run_grad<DT, 1, 4, VEC>(a, r, st);
+            case 8: return run_grad<DT, 2, 4, VEC>(a, r, st);
+            case 16: return run_grad<DT, 4, 4, VEC>(a, r, st);
+            case 32: return run_grad<DT, 4, 8, VEC>(a, r, st);
+            default: return run_grad<DT, 8, 8, VEC>(a, r, st);
         }
     }
     switch (NP) {
