@@ -162,6 +162,7 @@ void fill_scan(const aud_scan_params* p, const aud::ScanRoute& r, aud::ScanArgs*
     a->bi = p->b_item, a->br = p->b_row, a->ci = p->c_item, a->cr = p->c_row, a->yi = p->dy_item, a->yr = p->dy_row;
     a->chunks = r.chunks;
     a->chunk_tiles = r.chunk_tiles;
+    a->fold = r.fold;
 }
 
 }  // namespace

@@ -168,11 +168,12 @@ struct ScanArgs {
     float* part;                     // workspace: [B * chunks][N + 2][D]
     int B, L, Dn, G, N, softplus;
     int64_t ui, ur, ei, er, zi, zr, yi, yr, bi, br, ci, cr;  // item / row strides of u, delta, z, dy, Bm, Cm
-    int chunks, chunk_tiles;
+    int chunks, chunk_tiles, fold;
 };
 struct ScanRoute {
     int chunks, chunk_tiles;  // the time axis in `chunks` runs of chunk_tiles tiles, scanned side by side and joined
     int blocks;               // blocks of 64 channels a group has
+    bool fold;                // few chunks: each walks the ones in front of it, instead of a kernel that joins them
 };
 int scan_padded_states(int N);
 ScanRoute scan_route(int B, int L, int D, int G, int N, bool grad);

@@ -25,8 +25,8 @@ namespace {
 
 constexpr int kNT = 256, kT = kScanTile, kCh = 64;
 constexpr int kMaxChunks = 64, kJoinThreads = 64;
-// Up to 8 chunks a workgroup walks the ones in front of its own; with more that reads too much (16 chunks, 64 workgroups of
-// channels: 9 us more in the second scan) and a kernel between the scans (5 us) joins them.
+// Up to 8 chunks (16 where the card is not full) a workgroup walks the ones in front of its own; with more that reads too much
+// (16 chunks, 64 workgroups of channels: 9 us more in the second scan) and a kernel between the scans (5 us) joins them.
 constexpr int kFoldChunks = 8;
 
 #if defined(__clang__)
@@ -185,7 +185,7 @@ __device__ __forceinline__ void chunk_state(const ScanArgs& a, const Where& at, 
     const float* s = a.sums + int64_t(at.b) * a.chunks * per + d;
     const float* dt = a.sums + int64_t(a.B) * a.chunks * per + int64_t(at.b) * a.chunks * a.Dn + d;
     if (!live) return;
-    if (a.chunks > kFoldChunks) {  // k_scan_join has been over the table
+    if (!a.fold) {  // k_scan_join has been over the table
         const int64_t slot = BACK ? at.chunk + 1 : at.chunk;
 #pragma unroll
         for (int i = 0; i < NW; ++i)
@@ -856,7 +856,7 @@ hipError_t run(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     if (a.chunks > 1) {
         const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 1>), first, wg, lds1, st, a, r.blocks);
-        if (a.chunks > kFoldChunks) {
+        if (!a.fold) {
             const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
             hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<false>), dim3(join), dim3(kJoinThreads), 0, st, a);
         }
@@ -874,7 +874,7 @@ hipError_t run_grad(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     if (a.chunks > 1) {
         const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, W, VEC, 1>), first, dim3(64 * W), lds1, st, a, r.blocks);
-        if (a.chunks > kFoldChunks) {
+        if (!a.fold) {
             const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
             hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<true>), dim3(join), dim3(kJoinThreads), 0, st, a);
         }
@@ -922,16 +922,19 @@ int scan_padded_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : 
 // y); an uncut one keeps one workgroup a CU and needs enough of them.  Measured at 2048 steps of 64-channel workgroups
 // (bfloat16, 16 states, MI355X): 192 workgroups 190 us uncut, 217 / 216 / 220 us in 4 / 8 / 16 chunks; 64 workgroups 44 us of
 // kernels in 16 chunks, 46 in 8, 78 in 4.  So: uncut from 170 workgroups on, else about 512 workgroups, chunks of four tiles at
-// least.  The gradients (two workgroups a CU): the same, up to 1024 workgroups.
-ScanRoute scan_route(int B, int L, int D, int G, int, bool grad) {
+// least.  A tile of the gradients takes three times as long: chunks of two
+// tiles there (3 x 501 steps of 2 x 36 channels, values and gradients: 44 us, with four tiles 52).
+ScanRoute scan_route(int B, int L, int D, int G, int N, bool grad) {
     ScanRoute r{};
     r.blocks = (D / G + kCh - 1) / kCh;
     const int tiles = L > 0 ? (L + kT - 1) / kT : 1;
-    const int64_t wgs = int64_t(B) * G * r.blocks, want = grad ? 1024 : 512;
-    int64_t chunks = wgs >= (grad ? 400 : 170) ? 1 : (want + wgs - 1) / wgs;
-    chunks = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(chunks, kMaxChunks), tiles / 4));
+    const bool wide = scan_padded_states(N) > 16;
+    const int64_t wgs = int64_t(B) * G * r.blocks, want = 512, uncut = !grad ? 170 : wide ? 200 : 400;
+    int64_t chunks = wgs >= uncut || wgs == 0 ? 1 : want / wgs;  // (rounded down: one workgroup too many costs a whole round)
+    chunks = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(chunks, kMaxChunks), tiles / (grad ? 2 : 4)));
     r.chunk_tiles = int((tiles + chunks - 1) / chunks);
     r.chunks = (tiles + r.chunk_tiles - 1) / r.chunk_tiles;
+    r.fold = r.chunks <= kFoldChunks || (r.chunks <= 2 * kFoldChunks && wgs * r.chunks <= 256);
     return r;
 }
 int64_t scan_sums_floats(const ScanRoute& r, int B, int D, int N) { return r.chunks > 1 ? int64_t(B) * r.chunks * (N + 1) * D : 0; }
