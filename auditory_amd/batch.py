@@ -102,8 +102,8 @@ class BatchProcessor:
         weight, bias [channels] and act.  Beside kwta() the other way from the raw maps to activations; for training use
         auditory_amd.norm, which has the gradients."""
         from . import norm
-        n, channels = maps.shape[0], maps[0, 0, 0].numel() if maps.dim() > 3 else maps.shape[-1]
-        flat = maps.reshape(n, -1, channels)
+        n, py, px = maps.shape[:3]
+        flat = maps.reshape(n, py * px, int(np.prod(maps.shape[3:])))
         got = norm.group_norm(flat, groups, weight, bias, eps, act, lengths, want_stats=want_stats)
         return (got[0].view(maps.shape), got[1]) if want_stats else got.view(maps.shape)
 
@@ -118,7 +118,7 @@ class BatchProcessor:
         """a feature map [n, PY, PX, ...channels] as sequences over time, one a band: [n * PY, PX, channels] (no copy) -- what
         auditory_amd.scan's operators take"""
         n, py, px = maps.shape[:3]
-        return maps.reshape(n * py, px, -1)
+        return maps.reshape(n * py, px, int(np.prod(maps.shape[3:])))
 
     def process_sndenv(self, sig, items_dev, n_items, pools_y, pools_x, params, state=None):
         """ProcessSegment + ApplyGabor with Kwta.On for every item, device-resident end to end:

@@ -9,6 +9,7 @@ namespace {
 
 constexpr int64_t kMaxElements = int64_t(1) << 40;
 constexpr int32_t kMaxRows = 1 << 30;  // rows of an item: a tile behind them still counts in 32 bits
+constexpr int32_t kMaxChannels = 1 << 24;
 constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
 
 // the context's device for the length of a call; the caller's current device is put back
@@ -103,7 +104,7 @@ const char* conv_bad(const aud_conv_params* p, bool grad) {
     if (!p) return "null parameters";
     if (!known_type(p->dtype)) return "dtype must be AUD_F32, AUD_BF16 or AUD_F16";
     if (p->act != AUD_ACT_NONE && p->act != AUD_ACT_SILU) return "the convolution's activation is AUD_ACT_NONE or AUD_ACT_SILU";
-    if (p->n_items < 0 || p->steps < 0 || p->steps > kMaxRows || p->channels < 1) return "bad shape";
+    if (p->n_items < 0 || p->steps < 0 || p->steps > kMaxRows || p->channels < 1 || p->channels > kMaxChannels) return "bad shape";
     if (p->taps < 1 || p->taps > 4) return "taps must be 1 to 4";
     if (int64_t(p->n_items) * p->steps > kMaxElements / p->channels) return "tensor too large";
     const Input x{nullptr, p->n_items, p->steps, p->channels, p->x_item, p->x_row};
@@ -117,7 +118,7 @@ int64_t conv_tiles(const aud_conv_params* p, int T) { return p->steps > 0 ? (int
 const char* scan_bad(const aud_scan_params* p, bool gated, bool grad) {
     if (!p) return "null parameters";
     if (!known_type(p->dtype)) return "dtype must be AUD_F32, AUD_BF16 or AUD_F16";
-    if (p->n_items < 0 || p->steps < 0 || p->steps > kMaxRows || p->channels < 1 || p->groups < 1) return "bad shape";
+    if (p->n_items < 0 || p->steps < 0 || p->steps > kMaxRows || p->channels < 1 || p->channels > kMaxChannels || p->groups < 1) return "bad shape";
     if (p->channels % p->groups) return "channels must be a multiple of groups";
     if (p->states < 1 || p->states > 64) return "states must be 1 to 64";
     if (int64_t(p->n_items) * (p->steps > 0 ? p->steps : 1) > kMaxElements / (int64_t(p->channels) * p->states)) return "tensor too large";

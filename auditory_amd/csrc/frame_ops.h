@@ -2,6 +2,9 @@
 // their activations (float32, bfloat16, float16 -- parameters, statistics, states and every sum are float32), packed loads
 // and stores, the activation functions with their derivatives, and the launch descriptors.
 #pragma once
+#include <algorithm>
+#include <atomic>
+
 #include "kernels.h"
 
 namespace aud {
@@ -90,6 +93,20 @@ __device__ __forceinline__ float act_slope(float p) {
     } else if constexpr (ACT == AUD_ACT_GELU)
         return 0.5f * (1.f + erff(p * 0.70710678118654752f)) + p * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * p * p);
     else return 1.f;
+}
+
+// more than 64 KB of dynamic LDS has to be allowed, per kernel and device: once
+template <auto kernel>
+hipError_t allow_lds(size_t bytes) {
+    static std::atomic<uint64_t> allowed{0};
+    if (bytes <= 64 * 1024) return hipSuccess;
+    int device = 0;
+    if (hipError_t e = hipGetDevice(&device)) return e;
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (allowed.load(std::memory_order_acquire) & bit) return hipSuccess;
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    if (e == hipSuccess) allowed.fetch_or(bit, std::memory_order_release);
+    return e;
 }
 
 // rows of an item that count: lengths[b] held to [0, rows]; rows where there is no table

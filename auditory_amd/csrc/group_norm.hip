@@ -246,17 +246,24 @@ __global__ void __launch_bounds__(kItemThreads) k_norm_held(NormArgs a) {
             part[i] += x[j][i];
         }
     }
-    // twice: the sum of every group, by way of LDS -> stats[2 g + which]
+    // twice: the sum of every group, by way of LDS -> stats[2 g + which].  Where the packs of a row divide the wave, its rows are
+    // added among the lanes first
+    const bool fold = l.cols <= 64 && (l.cols & (l.cols - 1)) == 0;
+    const int runs = fold ? NT / 64 : l.lanes, run = fold ? int(threadIdx.x) >> 6 : l.r;
     auto sum_groups = [&](int which) {
-        if (mine) {
+        if (fold)
+            for (int s = l.cols; s < 64; s <<= 1)
 #pragma unroll
-            for (int i = 0; i < V; ++i) entries[l.r * a.C + l.c * V + i] = part[i];
+                for (int i = 0; i < V; ++i) part[i] += __shfl_xor(part[i], s);
+        if (mine && (!fold || int(threadIdx.x & 63) < l.cols)) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) entries[run * a.C + l.c * V + i] = part[i];
         }
         __syncthreads();
         for_groups<NT>(a.G, [&](int g, int lane, int q, bool there) {
             const int dr = q / cg, dc = q - dr * cg, r0 = lane / cg;
             float s = 0.f;
-            for (int r = r0, c = lane - r0 * cg; r < l.lanes;) {
+            for (int r = r0, c = lane - r0 * cg; r < runs;) {
                 s += entries[r * a.C + g * cg + c];
                 r += dr, c += dc;
                 if (c >= cg) c -= cg, ++r;
@@ -580,11 +587,6 @@ __global__ void __launch_bounds__(kCsCols * kCsLanes) k_column_sums(const float*
     }
 }
 
-template <typename K>
-hipError_t allow_lds(K kernel, size_t bytes) {
-    if (bytes <= 64 * 1024) return hipSuccess;
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-}
 inline size_t entries_of(int nt, int V, int C) { return size_t(2) * size_t(std::max(nt * V, C)); }
 
 template <int DT, int V, int ACT>
@@ -592,19 +594,19 @@ hipError_t run(const NormArgs& a, const NormRoute& r, hipStream_t st) {
     const int packs = a.C / V;
     if (r.one_wg && packs <= kItemThreads && int64_t(a.S) <= 4 * (kItemThreads / packs)) {
         const size_t lds = (2 * size_t(a.G) + size_t(kItemThreads / packs) * a.C) * 4;
-        if (hipError_t e = allow_lds(&k_norm_held<DT, V, ACT>, lds)) return e;
+        if (hipError_t e = allow_lds<&k_norm_held<DT, V, ACT>>(lds)) return e;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_held<DT, V, ACT>), dim3(unsigned(a.B)), dim3(kItemThreads), lds, st, a);
         return hipGetLastError();
     }
     if (r.one_wg) {
         const size_t lds = (2 * size_t(a.G) + entries_of(kItemThreads, V, a.C)) * 4;
-        if (hipError_t e = allow_lds(&k_norm_item<DT, V, ACT>, lds)) return e;
+        if (hipError_t e = allow_lds<&k_norm_item<DT, V, ACT>>(lds)) return e;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_item<DT, V, ACT>), dim3(unsigned(a.B)), dim3(kItemThreads), lds, st, a);
         return hipGetLastError();
     }
     const dim3 grid(unsigned(a.chunks) * unsigned(a.B)), wg(kChunkThreads);
     const size_t lds = (2 * size_t(a.G) + entries_of(kChunkThreads, V, a.C)) * 4;
-    if (hipError_t e = allow_lds(&k_norm_chunk<DT, V>, lds)) return e;
+    if (hipError_t e = allow_lds<&k_norm_chunk<DT, V>>(lds)) return e;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_chunk<DT, V>), grid, wg, lds, st, a);
     if (r.join) {
         const unsigned join = unsigned((int64_t(a.B) * a.G + kChunkThreads - 1) / kChunkThreads);
@@ -620,7 +622,7 @@ template <int DT, int V, int ACT>
 hipError_t run_grad(const NormArgs& a, const NormRoute& r, hipStream_t st) {
     if (r.one_wg) {
         const size_t lds = (4 * size_t(a.G) + 2 * size_t(a.C) + entries_of(kItemThreads, V, a.C)) * 4;
-        if (hipError_t e = allow_lds(&k_norm_grad_item<DT, V, ACT>, lds)) return e;
+        if (hipError_t e = allow_lds<&k_norm_grad_item<DT, V, ACT>>(lds)) return e;
         hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_grad_item<DT, V, ACT>), dim3(unsigned(a.B)), dim3(kItemThreads), lds, st, a);
         if (hipError_t e = hipGetLastError()) return e;
         if (a.B == 1 || (!a.dweight && !a.dbias)) return hipSuccess;
@@ -628,7 +630,7 @@ hipError_t run_grad(const NormArgs& a, const NormRoute& r, hipStream_t st) {
     }
     const unsigned work = unsigned(a.chunks) * unsigned(a.B);
     const size_t lds = (2 * size_t(a.G) + 2 * size_t(a.C) + entries_of(kChunkThreads, V, a.C)) * 4;
-    if (hipError_t e = allow_lds(&k_norm_grad_chunk<DT, V, ACT>, lds)) return e;
+    if (hipError_t e = allow_lds<&k_norm_grad_chunk<DT, V, ACT>>(lds)) return e;
     hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_grad_chunk<DT, V, ACT>), dim3(work), dim3(kChunkThreads), lds, st, a);
     const unsigned join = unsigned(a.B) * unsigned((2 * a.C + kJoinCols - 1) / kJoinCols);
     hipLaunchKernelGGL(k_norm_grad_join, dim3(join), dim3(kJoinCols * kJoinLanes), size_t(kJoinCols) * kJoinLanes * 4, st, a);

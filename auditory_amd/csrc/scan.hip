@@ -835,11 +835,6 @@ __global__ void __launch_bounds__(kNT) k_scan_bc(ScanArgs a, int blocks) {
     static_cast<typename Elem<DT>::raw*>(i < n ? a.dB : a.dC)[o] = Elem<DT>::down(s);
 }
 
-template <typename K>
-hipError_t allow_lds(K kernel, size_t bytes) {
-    if (bytes <= 64 * 1024) return hipSuccess;
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
-}
 
 template <int DT>
 void run_table(const ScanArgs& a, int NP, int NW, hipStream_t st) {
@@ -851,7 +846,7 @@ template <int DT, int NW, int W, bool VEC>
 hipError_t run(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     const dim3 grid(unsigned(int64_t(a.B) * a.chunks * a.G * r.blocks)), wg(64 * W);
     const size_t lds1 = size_t(4) * kT * kCh * 4, lds3 = lds1 + size_t(2) * W * kT * kCh * 4;
-    if (hipError_t e = allow_lds(&k_scan<DT, NW, W, VEC, 3>, lds3)) return e;
+    if (hipError_t e = allow_lds<&k_scan<DT, NW, W, VEC, 3>>(lds3)) return e;
     run_table<DT>(a, NW * W, NW, st);
     if (a.chunks > 1) {
         const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));
@@ -869,7 +864,7 @@ hipError_t run_grad(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     constexpr int NP = W * NW;
     const dim3 grid(unsigned(int64_t(a.B) * a.chunks * a.G * r.blocks));
     const size_t lds1 = size_t(2) * kT * kCh * 4, lds3 = size_t(3 * kT * kCh + 2 * kT * NP + 3 * W * kT * kCh) * 4;
-    if (hipError_t e = allow_lds(&k_scan_grad<DT, NW, W, VEC, 3>, lds3)) return e;
+    if (hipError_t e = allow_lds<&k_scan_grad<DT, NW, W, VEC, 3>>(lds3)) return e;
     run_table<DT>(a, NP, NW, st);
     if (a.chunks > 1) {
         const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));

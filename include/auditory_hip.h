@@ -509,7 +509,7 @@ int aud_kwta_batch_host(aud_ctx* ctx, const aud_kwta_params* k, const float* raw
 
 /* group norm: x [n_items, rows, channels], `groups` groups of neighbouring channels, each normalised over rows x its channels
  * (the biased variance), then weight, bias and the activation.  1 <= channels <= 4096, a multiple of groups;
- * eps > 0; at most 2^30 rows or steps in this and the following. */
+ * eps > 0; at most 2^30 rows or steps in this and the following, and 2^24 channels in those. */
 typedef struct {
     int32_t dtype, act, n_items, rows, channels, groups;
     float eps;
@@ -546,6 +546,7 @@ int aud_causal_conv_grad_dev(aud_ctx* ctx, const aud_conv_params* p, const void*
 /* selective scan: u, delta, z [n_items, steps, channels], B, C [n_items, steps, groups, states] (groups and states
  * contiguous; a group's B and C serve channels / groups neighbouring channels), A float32 [channels, states], D and
  * delta_bias float32 [channels] or NULL, z NULL for no gate.  1 <= states <= 64; channels a multiple of groups.
+ * A, and the states, must be finite.
  *   dt = softplus(delta + delta_bias) (softplus = 0: without it);  h = exp(dt A) h + dt u B;  y = (sum h C + D u) silu(z)
  * state, state_out float32 [n_items, channels, states]: the state in front of the first frame (NULL: zeros) and behind the
  * last of each item.  steps = 1 is the streaming form: one launch, no workspace. */
