@@ -117,8 +117,14 @@ int aud_host_register(aud_ctx* c, void* ptr, int64_t bytes) {
             if (lo < b.p + b.bytes && b.p < lo + bytes)
                 return fail(c, AUD_EINVAL, "aud_host_register: the range overlaps a block the context already holds");
     }
-    AUD_HIP(c, hipHostRegister(ptr, size_t(bytes), hipHostRegisterPortable | hipHostRegisterMapped));
     void* dev = nullptr;
+    if (hipHostRegister(ptr, size_t(bytes), hipHostRegisterPortable | hipHostRegisterMapped) != hipSuccess) {
+        // (some machines refuse it for memory that exists already: the range is noted without a device address, and results in
+        // it take the staging route)
+        (void)hipGetLastError();
+        c->host_blocks.push_back({static_cast<unsigned char*>(ptr), size_t(bytes), nullptr, true});
+        return AUD_OK;
+    }
     if (hipHostGetDevicePointer(&dev, ptr, 0) != hipSuccess || !dev) {
         (void)hipGetLastError();
         (void)hipHostUnregister(ptr);
@@ -134,8 +140,9 @@ int aud_host_unregister(aud_ctx* c, void* ptr) {
     HostCallGuard guard(c);  // (drains the stream: no kernel still writes the range)
     for (size_t i = 0; i < c->host_blocks.size(); ++i)
         if (c->host_blocks[i].p == ptr && c->host_blocks[i].registered) {
+            const bool pinned = c->host_blocks[i].dev != nullptr;
             c->host_blocks.erase(c->host_blocks.begin() + long(i));
-            (void)hipHostUnregister(ptr);
+            if (pinned) (void)hipHostUnregister(ptr);
             return AUD_OK;
         }
     return fail(c, AUD_EINVAL, "aud_host_unregister: not a range of aud_host_register");

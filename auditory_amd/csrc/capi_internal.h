@@ -33,7 +33,8 @@ struct aud_ctx {
     hipEvent_t pin_ev[8] = {nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
     // aud_host_alloc / aud_host_register: pinned, device-visible host memory the caller keeps result tensors in (under
     // host_mutex).  `dev` is the address the device uses for `p` (the same for aud_host_alloc memory; what
-    // hipHostGetDevicePointer says for a registered range, e.g. a shared mapping several processes write their shards into)
+    // hipHostGetDevicePointer says for a registered range, e.g. a shared mapping several processes write their shards into; null
+    // for a range the runtime refused to register)
     struct HostBlock {
         unsigned char* p;
         size_t bytes;
@@ -293,11 +294,12 @@ inline int fetch_widened(aud_ctx* c, const float* d_src, const WidenPart* parts,
     return AUD_OK;
 }
 
-// the aud_host_alloc / aud_host_register block of the context that holds [p, p + bytes), or null (the caller holds host_mutex)
+// the device-visible aud_host_alloc / aud_host_register block of the context that holds [p, p + bytes), or null (the caller holds
+// host_mutex)
 inline const aud_ctx::HostBlock* find_host_block(const aud_ctx* c, const void* p, size_t bytes) {
     const unsigned char* q = static_cast<const unsigned char*>(p);
     for (const auto& b : c->host_blocks)
-        if (q >= b.p && q + bytes <= b.p + b.bytes) return &b;
+        if (b.dev && q >= b.p && q + bytes <= b.p + b.bytes) return &b;
     return nullptr;
 }
 inline bool in_host_block(const aud_ctx* c, const void* p, size_t bytes) { return find_host_block(c, p, bytes) != nullptr; }
