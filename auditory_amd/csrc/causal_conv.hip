@@ -5,6 +5,9 @@
 //
 // A thread owns a pack of channels and walks T steps with the last K - 1 inputs in registers: every input is read once, but
 // for the K - 1 in front of a run.  Rows at and behind lengths[b] are not read; their results are zero.
+//
+// Memory bounds it: 8 x 2048 x 1536 bfloat16, K = 4, 23 us for 101 MB (4.3 TB/s; a copy reaches 5.2).  The loads of eight steps are
+// sent off together (one after the other, behind each other's stores: 28.7 us).
 #include "frame_ops.h"
 
 namespace aud {

@@ -8,6 +8,15 @@
 // and a sum of squared distances from it; those are joined (rows, channels, chunks of rows) by
 //   M2 = sum M2_i + n_i (m_i - m)^2, which has no cancellation, so a level far from zero costs nothing.
 // Rows at and behind lengths[b] are not read; their results are zero.
+//
+// Three routes by the size of an item.  Up to four packs a thread it stays in one workgroup's registers: read once, one launch
+// (256 x 352 x 16 float32: 6.6 us, floor 2.2; launch and the two trips through LDS are the rest).  Up to 32 KB (128 KB, 1 MB
+// with 256, 1024 items and more) one workgroup reads it twice.  Else chunks of rows in about 512 workgroups: moments of the chunks,
+// then every workgroup joins its item's and writes (gradients: channel sums, joined per item, then dx, the parameters' sums by
+// workgroups of their own behind them).  Memory bounds that route: 16 x 4096 x 512 bfloat16 forward 15 + 28 us (67 MB read, then 134
+// moved), gradients 28 + 5 + 36 us (134, then 201 MB), 109 us a pass on inputs that the Infinity Cache holds, 123 on others, where
+// one sweep of everything would be 65; an item of 4 MB is more than a CU holds, and workgroups that wait for one another inside a
+// launch are not used here.
 #include "frame_ops.h"
 
 namespace aud {
@@ -691,8 +700,9 @@ NormRoute norm_route(int dtype, int B, int S, int C, int G, int align, bool) {
     r.chunks = 1;
     r.chunk_rows = S;
     if (!r.one_wg) {
-        // about a thousand workgroups, at least 8 KB of input each
-        int64_t chunks = std::min<int64_t>((1024 + B - 1) / B, kMaxChunks);
+        // about 512 workgroups, two a CU, at least 8 KB of input each (16 x 4096 x 512 bfloat16, values and gradients: 110 us;
+        // 256 workgroups 116, 768 114, 1024 118, 2048 145)
+        int64_t chunks = std::min<int64_t>((512 + B - 1) / B, kMaxChunks);
         chunks = std::max<int64_t>(1, std::min<int64_t>(chunks, std::min<int64_t>(S, bytes / 8192)));
         r.chunk_rows = int((S + chunks - 1) / chunks);
         r.chunks = (S + r.chunk_rows - 1) / r.chunk_rows;

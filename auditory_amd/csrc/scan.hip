@@ -18,6 +18,13 @@
 // state out from those, h' = exp(A sum dt) h + (final state) chunk by chunk, and is scanned from there.
 //
 // Steps at and behind lengths[b] have dt = 0: the state stays, y is zero, and what the inputs hold there has no effect.
+//
+// The vector pipe bounds it, not memory: a state and step is one exponential (8 cycles of a SIMD) and four products and fused
+// products (4 cycles each), a channel and step about 75 more instructions (softplus, gate, conversions, the sum over the waves).
+// 8 x 2048 x 1536, 16 states, bfloat16: 187 us, 204 MB (floor 40 us); 192 workgroups, one a CU, whose SIMDs issue vector
+// instructions 79 % of the time.  Gradients, 4 x 2048 x 1024: 42 us the first scan, 135 the second (78 %), of 268 for values and
+// gradients.  What was measured on the way there: B and C broadcast from LDS 243 us; scalar loads without a group in hand 638, as
+// runs of 64 bytes a group ahead 207; one barrier a tile instead of two 190; both elements of a thread side by side 186.
 #include "frame_ops.h"
 
 namespace aud {
