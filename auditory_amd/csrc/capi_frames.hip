@@ -30,13 +30,15 @@ struct OnDevice {
 int elem_bytes(int dtype) { return dtype == AUD_F32 ? 4 : 2; }
 bool known_type(int dtype) { return dtype == AUD_F32 || dtype == AUD_BF16 || dtype == AUD_F16; }
 
-// an input [items, rows, width] with its strides: rows must not overlap one another, items neither
+// an input [items, rows, width] with its strides: no two elements in one place, items or rows outermost
 struct Input {
     const void* p;
     int64_t items, rows, width, item, row;
     bool strides_ok() const {
-        if (rows > 1 && row < width) return false;
-        return items <= 1 || rows == 0 || item >= (rows - 1) * row + width;
+        if (items == 0 || rows == 0) return true;
+        if (rows > 1 && (row < width || row > kMaxElements / (rows - 1))) return false;
+        if (items > 1 && (item < width || item > kMaxElements / (items - 1))) return false;
+        return items <= 1 || rows <= 1 || item >= (rows - 1) * row + width || row >= (items - 1) * item + width;
     }
     // bytes from p to the end of the last element
     int64_t span(int e) const { return items && rows && width ? ((items - 1) * item + (rows - 1) * row + width) * e : 0; }
@@ -91,7 +93,7 @@ const char* norm_bad(const aud_norm_params* p, bool grad) {
     if (int64_t(p->n_items) * p->rows > kMaxElements / p->channels) return "tensor too large";
     const Input x{nullptr, p->n_items, p->rows, p->channels, p->x_item, p->x_row};
     const Input d{nullptr, p->n_items, p->rows, p->channels, p->dy_item, p->dy_row};
-    if (!x.strides_ok() || (grad && !d.strides_ok())) return "strides make rows or items overlap";
+    if (!x.strides_ok() || (grad && !d.strides_ok())) return "strides make rows or items overlap, or reach too far";
     return nullptr;
 }
 // (the route goes by sizes alone, so that the workspace has one size whatever the alignment)
@@ -109,7 +111,7 @@ const char* conv_bad(const aud_conv_params* p, bool grad) {
     if (int64_t(p->n_items) * p->steps > kMaxElements / p->channels) return "tensor too large";
     const Input x{nullptr, p->n_items, p->steps, p->channels, p->x_item, p->x_row};
     const Input d{nullptr, p->n_items, p->steps, p->channels, p->dy_item, p->dy_row};
-    if (!x.strides_ok() || (grad && !d.strides_ok())) return "strides make rows or items overlap";
+    if (!x.strides_ok() || (grad && !d.strides_ok())) return "strides make rows or items overlap, or reach too far";
     return nullptr;
 }
 int64_t conv_tiles(const aud_conv_params* p, int T) { return p->steps > 0 ? (int64_t(p->steps) + T - 1) / T : 1; }
@@ -126,9 +128,9 @@ const char* scan_bad(const aud_scan_params* p, bool gated, bool grad) {
     const Input in[] = {{nullptr, n, l, p->channels, p->u_item, p->u_row}, {nullptr, n, l, p->channels, p->delta_item, p->delta_row},
                         {nullptr, n, l, gn, p->b_item, p->b_row}, {nullptr, n, l, gn, p->c_item, p->c_row}};
     for (const Input& i : in)
-        if (!i.strides_ok()) return "strides make rows or items overlap";
+        if (!i.strides_ok()) return "strides make rows or items overlap, or reach too far";
     const Input z{nullptr, n, l, p->channels, p->z_item, p->z_row}, d{nullptr, n, l, p->channels, p->dy_item, p->dy_row};
-    if ((gated && !z.strides_ok()) || (grad && !d.strides_ok())) return "strides make rows or items overlap";
+    if ((gated && !z.strides_ok()) || (grad && !d.strides_ok())) return "strides make rows or items overlap, or reach too far";
     return nullptr;
 }
 aud::ScanRoute scan_route_of(const aud_scan_params* p, bool grad) {

@@ -152,11 +152,14 @@ __global__ void __launch_bounds__(kNT) k_conv_grad(ConvArgs a, int tiles) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) p = fmaf(w[i][k], win[k][i], p);
                 q[0][i] = d[i] * act_slope<ACT>(p);
-                const float mine = own ? q[0][i] : 0.f;
-                db[i] += mine;
-#pragma unroll
-                for (int k = 0; k < K; ++k) dw[k][i] = fmaf(mine, win[k][i], dw[k][i]);
             }
+            if (own)
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    db[i] += q[0][i];
+#pragma unroll
+                    for (int k = 0; k < K; ++k) dw[k][i] = fmaf(q[0][i], win[k][i], dw[k][i]);
+                }
 #pragma unroll
             for (int k = 0; k < K - 1; ++k)
 #pragma unroll

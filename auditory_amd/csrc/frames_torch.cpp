@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cstdint>
 #include <string>
 #include <tuple>
 
@@ -59,6 +60,8 @@ struct Call {
         }
         if (t.dim() != axes && t.dim() != other_axes)
             bad(std::string(name) + " must have " + std::to_string(axes) + " axes, it has " + std::to_string(t.dim()));
+        for (int64_t n : t.sizes())
+            if (n > INT32_MAX) bad(std::string(name) + " has an axis longer than 2^31 - 1: " + shape_text(t.sizes()));
     }
     bool fits(const at::Tensor& t, at::ScalarType type, Shape shape) const {
         return t.scalar_type() == type && t.sizes() == shape && t.device() == x.device();

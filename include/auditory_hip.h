@@ -493,7 +493,8 @@ int aud_kwta_batch_host(aud_ctx* ctx, const aud_kwta_params* k, const float* raw
  *  - dtype AUD_F32, AUD_BF16 or AUD_F16 is the type of the activations (x, y, dy, dx, u, delta, z, B, C, conv states);
  *    parameters, their gradients, statistics and scan states are float32, and so is every sum.
  *  - *_item / *_row are the distances, in elements, between items and between rows (positions, frames) of an input; the
- *    channels of a row are contiguous.  Outputs are contiguous.  Inputs of any alignment that their type allows are taken;
+ *    channels of a row are contiguous; items or rows may be outermost ([rows, items, channels] seen the other way round), but
+ *    no two elements in one place.  Outputs are contiguous.  Inputs of any alignment that their type allows are taken;
  *    16-byte aligned pointers and strides run faster.
  *  - lengths: int32 [n_items] in device memory, or NULL (every item is full).  Rows at and behind an item's length are
  *    padding: whatever they hold (NaN too) has no effect; outputs and gradients are written as zero there.  A value outside

@@ -422,3 +422,79 @@ def test_gpu_encoder_behind_the_gabor_maps(orc):
     F.scan_check(a, None, True, zero, torch.zeros_like(h), y, h_end, None)
     F.scan_check(a, None, True, zero, torch.zeros_like(h), torch.stack(ys, 1), h, None)
     plan.close()
+
+
+# ---- inputs laid out frames first, seen items first ------------------------------------------------------------------------
+
+def frames_first(dev):
+    m = F.Make(dev, 11, "bf16")
+    B, L, D, G, N = 3, 40, 32, 2, 8
+    lengths = m.lengths("mixed", B, L)
+
+    def both(*shape):
+        t = m.n(*shape)
+        return t, t.transpose(0, 1).contiguous().transpose(0, 1)
+
+    (x, xt), (dy, dyt), (dt, dtt), (z, zt) = (both(B, L, D) for _ in range(4))
+    (Bm, Bt), (Cm, Ct) = (both(B, L, G, N) for _ in range(2))
+    A, w = -(0.2 + m.u(D, N)), m.n(D, 3, f32=True)
+    y, st = norm.group_norm(x, 4, lengths=lengths, want_stats=True)
+    yt, stt = norm.group_norm(xt, 4, lengths=lengths, want_stats=True)
+    pairs = [(y, yt), (st, stt)]
+    pairs += zip(norm.group_norm_grad(dy, x, st, 4, lengths=lengths)[:1], norm.group_norm_grad(dyt, xt, st, 4, lengths=lengths)[:1])
+    pairs.append((scan.causal_conv(x, w, act="silu", lengths=lengths), scan.causal_conv(xt, w, act="silu", lengths=lengths)))
+    pairs += list(zip(scan.causal_conv_grad(dy, x, w, lengths=lengths), scan.causal_conv_grad(dyt, xt, w, lengths=lengths)))[:2]
+    (v, kept), (vt, _) = (scan.selective_scan(*a, A, *bc, z=g, softplus=True, lengths=lengths, keep=True)
+                          for a, bc, g in (((x, dt), (Bm, Cm), z), ((xt, dtt), (Bt, Ct), zt)))
+    pairs.append((v, vt))
+    got = scan.selective_scan_grad(dy, x, dt, A, Bm, Cm, kept, z=z, softplus=True, lengths=lengths)
+    gott = scan.selective_scan_grad(dyt, xt, dtt, A, Bt, Ct, kept, z=zt, softplus=True, lengths=lengths)
+    pairs += [(p, q) for p, q in zip(got, gott) if p is not None]
+    for i, (p, q) in enumerate(pairs):
+        assert q.is_contiguous() and torch.equal(p, q), i
+
+
+def test_emul_frames_first(emu):
+    frames_first("cpu")
+
+
+@gpu
+def test_gpu_frames_first():
+    frames_first("cuda:0")
+
+
+def infinite_input(dev):
+    """the weights' gradient of a run of frames that ends in an infinite input: infinite, not NaN"""
+    x, dy, w = torch.ones(1, 40, 4), torch.ones(1, 40, 4), torch.ones(4, 2)
+    for t in (7, 15, 31):
+        x[0, t] = float("inf")
+    g = scan.causal_conv_grad(dy.to(dev), x.to(dev), w.to(dev))
+    assert torch.isposinf(g.weight).all() and torch.equal(g.x.cpu()[0, :39], torch.full((39, 4), 2.0))
+
+
+def test_emul_conv_gradients_of_infinite_inputs(emu):
+    infinite_input("cpu")
+
+
+@gpu
+def test_gpu_conv_gradients_of_infinite_inputs():
+    infinite_input("cuda:0")
+
+
+def test_axes_past_32_bits_are_refused(emu):
+    wide = torch.zeros(1, 1, 1).expand(2 ** 31 + 1, 1, 1)
+    assert "2^31" in refused(norm.group_norm, wide, 1)
+    assert "2^31" in refused(norm.group_norm, wide.transpose(0, 1), 1)
+    assert "2^31" in refused(scan.causal_conv, wide, torch.zeros(1, 2))
+    assert "2^31" in refused(scan.causal_conv_step, wide[:, 0], torch.zeros(1, 1, 1), torch.zeros(1, 2))
+    assert "2^31" in refused(scan.selective_scan, wide, wide, torch.zeros(1, 2), torch.zeros(1, 1, 1, 2), torch.zeros(1, 1, 1, 2))
+
+
+def test_strides_that_reach_too_far_are_refused(emu):
+    p = capi.NormParams(dtype=capi.AUD_F32, act=0, n_items=2, rows=3, channels=4, groups=1, eps=1e-5, x_item=2 ** 62, x_row=4)
+    n = C.c_int64()
+    assert emu.aud_group_norm_workspace_bytes(C.byref(p), 0, C.byref(n)) == capi.AUD_EINVAL
+    p.x_item, p.x_row = 4, 8                   # frames first
+    assert emu.aud_group_norm_workspace_bytes(C.byref(p), 0, C.byref(n)) == capi.AUD_OK
+    p.x_item, p.x_row = 4, 7                   # the last channel of an item in the first of another
+    assert emu.aud_group_norm_workspace_bytes(C.byref(p), 0, C.byref(n)) == capi.AUD_EINVAL
