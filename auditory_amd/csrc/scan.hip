@@ -25,6 +25,8 @@
 // instructions 79 % of the time.  Gradients, 4 x 2048 x 1024: 42 us the first scan, 135 the second (78 %), of 268 for values and
 // gradients.  What was measured on the way there: B and C broadcast from LDS 243 us; scalar loads without a group in hand 638, as
 // runs of 64 bytes a group ahead 207; one barrier a tile instead of two 190; both elements of a thread side by side 186.
+#include <type_traits>
+
 #include "frame_ops.h"
 
 namespace aud {
@@ -259,46 +261,46 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     }
     const int first = at.chunk * a.chunk_tiles, end = first + a.chunk_tiles < tiles ? first + a.chunk_tiles : tiles;
     Raw<DT, E, VEC> ru{}, rd{}, rz{};
-    // addresses of this thread's channels in its row of the tile, moved on by 16 rows a tile (a row behind the last one is not
-    // looked at: the address stays where it is)
+    // addresses of this thread's channels in its row of the tile, moved on by 16 rows a tile (rows behind the last one: the last)
     typedef typename Elem<DT>::raw raw;
     const int cc = c < at.dn ? c : 0, left = at.dn - cc;
-    const int64_t row = first * kT + pt < a.L ? first * kT + pt : (a.L > 0 ? a.L - 1 : 0);
+    const int64_t row = first * kT + pt;
     const raw* pu = static_cast<const raw*>(a.u) + u0 + row * a.ur + cc;
     const raw* pd = static_cast<const raw*>(a.delta) + e0 + row * a.er + cc;
     const raw* pz = a.z ? static_cast<const raw*>(a.z) + z0 + row * a.zr + cc : pu;  // (no gate: read and not used)
-    const int64_t su = kT * a.ur, sd = kT * a.er, sz_ = a.z ? kT * a.zr : su;
-    auto fetch = [&] {
+    const int64_t su = kT * a.ur, sd = kT * a.er, sz = a.z ? kT * a.zr : su;
+    auto fetch = [&](int tile) {
+        if ((tile + 1) * kT > a.L) {  // (the last tile: the addresses are not moved on from here)
+            const int64_t over = tile * kT + pt < a.L ? 0 : tile * kT + pt - (a.L - 1);
+            pu -= over * a.ur, pd -= over * a.er, pz -= over * (a.z ? a.zr : a.ur);
+        }
         ru.load(pu, left);
         rd.load(pd, left);
         if (PASS == 3) rz.load(pz, left);
     };
-    auto advance = [&](int tile) {
-        if (tile * kT + pt < a.L) pu += su, pd += sd, pz += sz_;
-    };
     float* pk = a.kept ? a.kept + ((int64_t(at.b) * tiles + first) * a.N + wave * NW) * a.Dn + d : nullptr;
     raw* py = PASS == 3 ? static_cast<raw*>(a.y) + y0 + int64_t(first * kT + pt) * a.Dn : nullptr;
-    float u[E], z[E];  // of the tile that is being scanned
+    float u[2][E], z[2][E];  // of the tile that is being scanned, and of the next one
     auto stage = [&](int tile, int buf) {
         float step[2 * E], dt[E];
         const bool row_on = tile * kT + pt < len;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const bool on = row_on && c + i < at.dn;
-            u[i] = on ? ru.get(i) : 0.f;
-            z[i] = on ? rz.get(i) : 0.f;
+            u[buf][i] = ru.get(i);
+            z[buf][i] = rz.get(i);
             dt[i] = rd.get(i) + bias[i];
         }
         step_sizes(dt, a.softplus);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            step[2 * i] = row_on && c + i < at.dn ? dt[i] : 0.f;
-            step[2 * i + 1] = step[2 * i] * u[i];
+            const bool on = row_on && c + (VEC ? 0 : i) < at.dn;
+            step[2 * i] = on ? dt[i] : 0.f;
+            step[2 * i + 1] = on ? dt[i] * u[buf][i] : 0.f;
         }
         lds_write(lds + 2 * ((buf * kT + pt) * kCh + c), step);
     };
     if (first < end) {
-        fetch();
+        fetch(first);
         stage(first, 0);
     }
     __syncthreads();
@@ -308,10 +310,12 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     Vec next{};
     wait_loads();
     if (first < end) next.template load<true, PASS == 3>(bc);
-    for (int tile = first, buf = 0; tile < end; ++tile, buf ^= 1, bc += kT * 2 * NP) {
-        if (tile + 1 < end) {
-            advance(tile + 1);
-            fetch();
+    auto scan_tile = [&](int tile, auto which) {  // (a turn of the loop for each buffer: what belongs to one stays in its registers)
+        constexpr int buf = decltype(which)::value;
+        const bool more = tile + 1 < end;
+        if (more) {
+            pu += su, pd += sd, pz += sz;
+            fetch(tile + 1);
         }
         if (PASS == 3 && a.kept) {
 #pragma unroll
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
 #pragma unroll
             for (int k = 0; k < GS; ++k) st[k] = s_step[(buf * kT + k0 + k) * kCh + lane];
             ScalarTable ahead = bc + (k0 + GS) * 2 * NW;
-            if (k0 + GS == kT) ahead = tile + 1 < end ? bc + kT * 2 * NP : bc;  // (nothing behind the last tile: any address of the table)
+            if (k0 + GS == kT) ahead = more ? bc + kT * 2 * NP : bc;  // (nothing behind the last tile: any address of the table)
             wait_lds();
             next.template load<true, PASS == 3>(ahead);
             __builtin_amdgcn_sched_barrier(0);
@@ -342,16 +346,14 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
                 else sum_dt += st[k].x;
             }
         }
-        float su[E], sz[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) su[i] = u[i], sz[i] = z[i];
-        if (tile + 1 < end) stage(tile + 1, buf ^ 1);
+        bc += kT * 2 * NP;
+        if (more) stage(tile + 1, buf ^ 1);
         __syncthreads();
         const int t = tile * kT + pt;
         if (PASS == 3 && t < a.L) {
             float y[E];
 #pragma unroll
-            for (int i = 0; i < E; ++i) y[i] = skip[i] * su[i];
+            for (int i = 0; i < E; ++i) y[i] = skip[i] * u[buf][i];
 #pragma unroll
             for (int w = 0; w < W; ++w) {
                 float part[E];
@@ -361,12 +363,16 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
             }
             if (a.z)
 #pragma unroll
-                for (int i = 0; i < E; ++i) y[i] *= sz[i] * fast_sigmoid(sz[i]);
+                for (int i = 0; i < E; ++i) y[i] *= z[buf][i] * fast_sigmoid(z[buf][i]);
 #pragma unroll
             for (int i = 0; i < E; ++i) y[i] = t < len ? y[i] : 0.f;
             store_some<DT, E, VEC>(py, 0, c, at.dn, y);
         }
         if (PASS == 3) py += kT * a.Dn;
+    };
+    for (int tile = first; tile < end; tile += 2) {
+        scan_tile(tile, std::integral_constant<int, 0>{});
+        if (tile + 1 < end) scan_tile(tile + 1, std::integral_constant<int, 1>{});
     }
     if (!live) return;
     float* dt_sums = a.sums + int64_t(a.B) * a.chunks * a.N * a.Dn;
