@@ -577,24 +577,41 @@ __global__ void __launch_bounds__(64 * W, 2) k_scan_grad(ScanArgs a, int blocks)
     }
     const int first = at.chunk * a.chunk_tiles, end = first + a.chunk_tiles < tiles ? first + a.chunk_tiles : tiles;
     Raw<DT, E, VEC> ru{}, rd{}, rz{}, ry{};
+    // addresses of this thread's channels in its row of the tile, moved back by 16 rows a tile (rows behind the last one: the last)
     typedef typename Elem<DT>::raw raw;
     const int cc = c < at.dn ? c : 0, left = at.dn - cc;
+    const int64_t row = (end - 1) * kT + pt, over = row < a.L ? 0 : row - (a.L - 1);
+    const raw* pu = static_cast<const raw*>(a.u) + u0 + (row - over) * a.ur + cc;
+    const raw* pd = static_cast<const raw*>(a.delta) + e0 + (row - over) * a.er + cc;
+    const raw* pg = static_cast<const raw*>(a.dy) + g0 + (row - over) * a.yr + cc;
+    const raw* pz = a.z ? static_cast<const raw*>(a.z) + z0 + (row - over) * a.zr + cc : pg;  // (no gate: read and not used)
+    const int64_t su = kT * a.ur, sd = kT * a.er, sg = kT * a.yr, sz = a.z ? kT * a.zr : sg;
+    const int64_t step_o = int64_t(kT) * a.Dn;
+    const int lane_in = live ? lane : 0;
+    // (the same for all lanes: states in front of the tile, results of its first row)
+    const float* pk = PASS == 3 ? a.kept + ((int64_t(at.b) * tiles + (end - 1)) * a.N + wave * NW) * a.Dn + at.d0 : nullptr;
+    const unsigned lane_o = unsigned((int64_t(pt) * a.Dn + c) * int(sizeof(raw)));  // bytes: 16 rows of 2^24 channels at most
+    int64_t o_tile = o0 + int64_t(end - 1) * step_o;
+    const int64_t gn = int64_t(a.G) * a.N, table_bc = int64_t(a.B) * a.L * gn;
+    int64_t o_bc = (int64_t(at.b) * a.L + int64_t(end - 1) * kT) * gn + int64_t(at.g) * a.N;
     float h0[NW];  // the state in front of the tile
-    auto fetch = [&](int tile) {
-        const int64_t row = tile * kT + pt < a.L ? tile * kT + pt : a.L - 1;
-        if (PASS == 3) ru.load(static_cast<const raw*>(a.u) + u0 + row * a.ur + cc, left);
-        rd.load(static_cast<const raw*>(a.delta) + e0 + row * a.er + cc, left);
-        if (a.z) rz.load(static_cast<const raw*>(a.z) + z0 + row * a.zr + cc, left);
-        ry.load(static_cast<const raw*>(a.dy) + g0 + row * a.yr + cc, left);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) h0[i] = 0.f;
+    auto fetch = [&] {
+        if (PASS == 3) ru.load(pu, left);
+        rd.load(pd, left);
+        rz.load(pz, left);
+        ry.load(pg, left);
         if (PASS == 3)
 #pragma unroll
-            for (int i = 0; i < NW; ++i) {
-                const int n = wave * NW + i;
-                h0[i] = live && n < a.N ? a.kept[((int64_t(at.b) * tiles + tile) * a.N + n) * a.Dn + d] : 0.f;
-            }
+            for (int i = 0; i < NW; ++i)
+                if (wave * NW + i < a.N) h0[i] = pk[int64_t(i) * a.Dn + lane_in];
     };
     wait_loads();
-    if (first < end) fetch(end - 1);
+    if (first < end) {
+        fetch();
+        pu += over * a.ur, pd += over * a.er, pg += over * a.yr, pz += over * (a.z ? a.zr : a.yr);
+    }
     ScalarTable bc = (ScalarTable)(a.table + ((int64_t(at.b) * a.G + at.g) * tiles + (end - 1)) * kT * 2 * NP + wave * kT * 2 * NW);
     for (int tile = end - 1; tile >= first; --tile, bc -= kT * 2 * NP) {
         const int t0 = tile * kT, t = t0 + pt;
@@ -602,7 +619,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_scan_grad(ScanArgs a, int blocks)
         float u[E], z[E], dy[E], arg[E], dt[E], f[E], dtu[E], hs0[NW];
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const bool there = on && c + i < at.dn;
+            const bool there = on && c + (VEC ? 0 : i) < at.dn;
             u[i] = there ? ru.get(i) : 0.f;
             z[i] = there ? rz.get(i) : 0.f;
             dy[i] = there ? ry.get(i) : 0.f;
@@ -616,16 +633,20 @@ __global__ void __launch_bounds__(64 * W, 2) k_scan_grad(ScanArgs a, int blocks)
             for (int i = 0; i < E; ++i) f[i] *= z[i] * fast_sigmoid(z[i]);
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            if (!(on && c + i < at.dn)) dt[i] = 0.f;
+            if (!(on && c + (VEC ? 0 : i) < at.dn)) dt[i] = 0.f;
             dtu[i] = dt[i] * u[i];
         }
         lds_write(s_dt + pt * kCh + c, dt);
         lds_write(s_f + pt * kCh + c, f);
         if (PASS == 3) lds_write(s_du + pt * kCh + c, dtu);
 #pragma unroll
-        for (int i = 0; i < NW; ++i) hs0[i] = h0[i];
+        for (int i = 0; i < NW; ++i) hs0[i] = live ? h0[i] : 0.f;
         __syncthreads();
-        if (tile > first) fetch(tile - 1);
+        if (tile > first) {
+            pu -= su, pd -= sd, pg -= sg, pz -= sz;
+            if (PASS == 3) pk -= int64_t(a.N) * a.Dn;
+            fetch();
+        }
         typedef Vectors<NW> Vec;
         constexpr int GS = Vec::GS;
         if constexpr (PASS == 1) {
@@ -780,27 +801,30 @@ __global__ void __launch_bounds__(64 * W, 2) k_scan_grad(ScanArgs a, int blocks)
                     if (!on) du[i] = dd[i] = dz[i] = 0.f;
                     sum_dd[i] += dd[i];
                 }
-                const int64_t o = o0 + int64_t(t) * a.Dn;
-                store_some<DT, E, VEC>(a.du, o, c, at.dn, du);
-                store_some<DT, E, VEC>(a.ddelta, o, c, at.dn, dd);
-                if (a.dz) store_some<DT, E, VEC>(a.dz, o, c, at.dn, dz);
+                auto put = [&](void* base, const float (&f)[E]) {
+                    store_some<DT, E, VEC>(reinterpret_cast<char*>(static_cast<raw*>(base) + o_tile) + lane_o, 0, 0, at.dn - c, f);
+                };
+                put(a.du, du);
+                put(a.ddelta, dd);
+                if (a.dz) put(a.dz, dz);
             }
+            o_tile -= step_o;
             // dB, dC of the tile, summed over this block's channels: partial sums where the group has more blocks
-            const int64_t table = int64_t(a.B) * a.L * a.G * a.N;
             for (int i = tid; i < kT * NP; i += 64 * W) {
                 const int k = i / NP, n = i % NP;
                 if (n >= a.N || t0 + k >= a.L) continue;
-                const int64_t o = ((int64_t(at.b) * a.L + t0 + k) * a.G + at.g) * a.N + n;
+                const int64_t o = k * gn + n;
                 const bool there = t0 + k < len;
                 const float vb = there ? s_db[i] : 0.f, vc = there ? s_dc[i] : 0.f;
                 if (blocks == 1) {
-                    static_cast<typename Elem<DT>::raw*>(a.dB)[o] = Elem<DT>::down(vb);
-                    static_cast<typename Elem<DT>::raw*>(a.dC)[o] = Elem<DT>::down(vc);
+                    (static_cast<raw*>(a.dB) + o_bc)[o] = Elem<DT>::down(vb);
+                    (static_cast<raw*>(a.dC) + o_bc)[o] = Elem<DT>::down(vc);
                 } else {
-                    a.part_bc[at.block * table + o] = vb;
-                    a.part_bc[(blocks + at.block) * table + o] = vc;
+                    (a.part_bc + at.block * table_bc + o_bc)[o] = vb;
+                    (a.part_bc + (blocks + at.block) * table_bc + o_bc)[o] = vc;
                 }
             }
+            o_bc -= kT * gn;
         }
     }
     if constexpr (PASS == 1) {
