@@ -20,11 +20,13 @@
 // Steps at and behind lengths[b] have dt = 0: the state stays, y is zero, and what the inputs hold there has no effect.
 //
 // The vector pipe bounds it, not memory: a state and step is one exponential (8 cycles of a SIMD) and four products and fused
-// products (4 cycles each), a channel and step about 75 more instructions (softplus, gate, conversions, the sum over the waves).
-// 8 x 2048 x 1536, 16 states, bfloat16: 187 us, 204 MB (floor 40 us); 192 workgroups, one a CU, whose SIMDs issue vector
-// instructions 79 % of the time.  Gradients, 4 x 2048 x 1024: 42 us the first scan, 135 the second (78 %), of 268 for values and
+// products (4 cycles each), a channel and step about 50 more instructions (softplus, gate, conversions, the sum over the waves).
+// 8 x 2048 x 1536, 16 states, bfloat16: 178 us, 204 MB (floor 40 us); 192 workgroups, one a CU, whose SIMDs issue vector
+// instructions 75 % of the time.  Gradients, 4 x 2048 x 1024: 41 us the first scan, 126 the second (82 %), of 255 for values and
 // gradients.  What was measured on the way there: B and C broadcast from LDS 243 us; scalar loads without a group in hand 638, as
-// runs of 64 bytes a group ahead 207; one barrier a tile instead of two 190; both elements of a thread side by side 186.
+// runs of 64 bytes a group ahead 207; one barrier a tile instead of two 190; both elements of a thread side by side 186; addresses
+// moved on by a tile, a turn of the loop for each LDS buffer 178.  Not taken: the steps' LDS reads a group ahead 182, the output of
+// a tile behind the next one's scan 192, groups of half the size 194; inputs that lie still in the caches change nothing.
 #include <type_traits>
 
 #include "frame_ops.h"
@@ -226,7 +228,7 @@ __device__ __forceinline__ void chunk_state(const ScanArgs& a, const Where& at, 
 // ---- values.  PASS 1: a chunk's final state from zero and its sum of dt; PASS 3: y.  W waves of NW states each ---------------
 // One barrier a tile: between two of them a wave runs its states over tile k, turns the inputs of tile k + 1 (on their way
 // while it ran) into steps and, at the next one's start, adds up and stores tile k.  Eight waves of two states (16 states)
-// against four of four: 190 / 275 us at 8 x 2048 x 1536, 16 waves of one: 199.
+// against four of four, when the whole took 190 us: 275 us at 8 x 2048 x 1536, 16 waves of one: 199.
 template <int DT, int NW, int W, bool VEC, int PASS>
 __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     constexpr int NP = W * NW, E = 16 / W, ROW = kCh / E;  // elements a thread loads and stores, threads a step
@@ -952,7 +954,7 @@ int scan_padded_states(int N) { return N <= 4 ? 4 : N <= 8 ? 8 : N <= 16 ? 16 : 
 
 // Chunks of the time axis.  A cut axis is scanned twice, which costs 1.7 times the instructions (the first pass has no C, z and
 // y); an uncut one keeps one workgroup a CU and needs enough of them.  Measured at 2048 steps of 64-channel workgroups
-// (bfloat16, 16 states, MI355X): 192 workgroups 190 us uncut, 217 / 216 / 220 us in 4 / 8 / 16 chunks; 64 workgroups 44 us of
+// (bfloat16, 16 states, MI355X, uncut 190 us then): 192 workgroups 217 / 216 / 220 us in 4 / 8 / 16 chunks; 64 workgroups 44 us of
 // kernels in 16 chunks, 46 in 8, 78 in 4.  So: uncut from 170 workgroups on, else about 512 workgroups, chunks of four tiles at
 // least.  A tile of the gradients takes three times as long: chunks of two
 // tiles there (3 x 501 steps of 2 x 36 channels, values and gradients: 44 us, with four tiles 52).
