@@ -1,5 +1,5 @@
 // C ABI of the feature-map and frame-sequence operators: argument checks, routes and launches (group_norm.hip,
-// causal_conv.hip, scan.hip).  Nothing here allocates, synchronises or keeps a pointer.
+// causal_conv.hip, scan.hip, scan_grad.hip).  Nothing here allocates, synchronises or keeps a pointer.
 #include "capi_internal.h"
 #include "frame_ops.h"
 

@@ -1,4 +1,4 @@
-// Shared by the feature-map and frame-sequence operators (group_norm.hip, causal_conv.hip, scan.hip): the element types of
+// Shared by the feature-map and frame-sequence operators (group_norm, causal_conv, scan, scan_grad .hip): the element types of
 // their activations (float32, bfloat16, float16 -- parameters, statistics, states and every sum are float32), packed loads
 // and stores, the activation functions with their derivatives, and the launch descriptors.
 #pragma once
@@ -180,7 +180,7 @@ struct ScanArgs {
     void *dB, *dC;                   // [B, L, G, N] contiguous
     float *dA, *dD, *ddelta_bias, *dstate;  // dD, ddelta_bias, dstate may be null
     float* table;                    // workspace: B and C in float32 [B, G, 16 tiles, 2, padded states]
-    float* sums;                     // workspace: chunk states [B, chunks, N, D] (scan.hip chunk_state), chunk step sums [B, chunks, D]
+    float* sums;                     // workspace: chunk states [B, chunks, N, D] (scan_common.h chunk_state), chunk step sums [B, chunks, D]
     float* part_bc;                  // workspace: [2][blocks of a group][B, L, G, N]
     float* part;                     // workspace: [B * chunks][N + 2][D]
     int B, L, Dn, G, N, softplus;
