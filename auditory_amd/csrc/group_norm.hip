@@ -25,12 +25,15 @@ namespace {
 constexpr int kItemThreads = 512, kChunkThreads = 256;
 constexpr int kMaxChunks = 256;
 
-template <int NT>
-struct Lanes {  // how a workgroup's threads lie on (rows, packs of channels) for packs [first, first + cols)
+// How a workgroup's threads lie on (rows, packs of channels) for packs [first, first + cols).  Where the packs take several sweeps
+// the last one has threads left over: they may take rows of their own (SPREAD) only if what the lanes of a pack hold is not joined
+// behind the sweeps -- the joins know one number of lanes, and their tables have room for NT packs of one sweep or C channels once.
+template <int NT, bool SPREAD>
+struct Lanes {
     int cols, lanes, r, c;
     __device__ __forceinline__ Lanes(int n_packs, int first) {
         cols = n_packs - first < NT ? n_packs - first : NT;
-        lanes = NT / cols;
+        lanes = SPREAD || n_packs <= NT ? NT / cols : 1;
         r = int(threadIdx.x) / cols;
         c = first + int(threadIdx.x) - r * cols;
         if (r >= lanes) r = 1 << 30;  // left over: no row is theirs
@@ -100,8 +103,8 @@ __device__ __forceinline__ void group_moments(const NormArgs& a, int b, int lo, 
     float *e_mean = entries, *e_m2 = entries + size;
     int width = a.C, lanes = 1;
     for (int first = 0; first < packs; first += NT) {
-        const Lanes<NT> l(packs, first);
-        lanes = l.lanes;  // (more than one only where all packs fit at once)
+        const Lanes<NT, false> l(packs, first);
+        lanes = l.lanes;  // (the same in every sweep)
         float k[V], s[V], ss[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) k[i] = s[i] = ss[i] = 0.f;
@@ -166,7 +169,7 @@ template <int DT, int V, int ACT, int NT>
 __device__ __forceinline__ void apply_rows(const NormArgs& a, int b, int lo, int hi, int rows, const float* stats) {
     const int packs = a.C / V, live = hi < rows ? hi : rows;
     for (int first = 0; first < packs; first += NT) {
-        const Lanes<NT> l(packs, first);
+        const Lanes<NT, true> l(packs, first);
         if (l.r >= l.lanes) continue;
         Affine<V> f;
         f.load(a, stats, l.c * V);
@@ -216,7 +219,7 @@ __global__ void __launch_bounds__(kItemThreads) k_norm_held(NormArgs a) {
     float* stats = reinterpret_cast<float*>(dyn_lds());  // [G, 2]
     float* entries = stats + 2 * a.G;                    // [lanes][C]
     const int b = blockIdx.x, rows = item_rows(a.lengths, b, a.S), packs = a.C / V, cg = a.C / a.G;
-    const Lanes<NT> l(packs, 0);
+    const Lanes<NT, false> l(packs, 0);
     const bool mine = l.r < l.lanes;
     const int64_t base = int64_t(b) * a.xi + int64_t(l.c) * V;
     float x[R][V];
@@ -387,7 +390,7 @@ __device__ __forceinline__ void channel_sums(const NormArgs& a, int b, int lo, i
     const int packs = a.C / V, size = NT * V > a.C ? NT * V : a.C;
     int lanes = 1;
     for (int first = 0; first < packs; first += NT) {
-        const Lanes<NT> l(packs, first);
+        const Lanes<NT, false> l(packs, first);
         lanes = l.lanes;
         if (l.r >= l.lanes) continue;
         Affine<V> f;
@@ -454,7 +457,7 @@ template <int DT, int V, int ACT, int NT>
 __device__ __forceinline__ void grad_rows(const NormArgs& a, int b, int lo, int hi, int rows, const float* stats, const float* gsum) {
     const int packs = a.C / V, live = hi < rows ? hi : rows;
     for (int first = 0; first < packs; first += NT) {
-        const Lanes<NT> l(packs, first);
+        const Lanes<NT, true> l(packs, first);
         if (l.r >= l.lanes) continue;
         Affine<V> f;
         f.load(a, stats, l.c * V);
