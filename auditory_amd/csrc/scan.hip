@@ -15,7 +15,8 @@
 //
 // Where items x channels leave the card idle, the time axis is cut into chunks: (1) every chunk but the last is scanned, the
 // first from the true state, the others from zero, for its final state and its sum of dt; (3) every chunk works its true
-// state out from those, h' = exp(A sum dt) h + (final state) chunk by chunk, and is scanned from there.
+// state out from those, h' = exp(A sum dt) h + (final state) chunk by chunk, and is scanned from there.  The decay of a chunk
+// may pass float32 (growing steps); its product with h is taken so that it does not.
 //
 // Steps at and behind lengths[b] have dt = 0: the state stays, y is zero, and what the inputs hold there has no effect.
 //

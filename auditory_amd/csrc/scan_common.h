@@ -52,6 +52,15 @@ __device__ __forceinline__ void wait_loads() {
 }
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// 2^x h + part, x the exponent of a whole run of steps.  A run of growing steps can pass float32 where its product with a small h
+// does not, and h = 0 stays 0 whatever it is multiplied by: what x has above 120 goes into h first, by powers of two.  (500: more
+// than that takes the smallest h there is past float32.)
+__device__ __forceinline__ float carried(float x, float h, float part) {
+    const float y = x > 500.f ? 500.f : x;
+    const int n = y > 120.f ? int(ceilf(y - 120.f)) : 0;
+    return fmaf(exp2_hw(y - float(n)), ldexpf(h, n), part);
+}
+
 struct Where {  // which channels, chunk and item a workgroup has
     int b, chunk, g, d0, dn, block;  // first channel, channels (<= 64), block within the group
     // (the first pass leaves the last chunk out, the gradients' first pass the first one)
@@ -192,7 +201,7 @@ __device__ __forceinline__ void chunk_state(const ScanArgs& a, const Where& at, 
         for (int j = 0; j < kAhead; ++j) {
             if (k + j >= count) break;
 #pragma unroll
-            for (int i = 0; i < NW; ++i) h[i] = k + j == 0 ? part[j][i] : fmaf(exp2_hw(sum[j] * A2[i]), h[i], part[j][i]);
+            for (int i = 0; i < NW; ++i) h[i] = k + j == 0 ? part[j][i] : carried(sum[j] * A2[i], h[i], part[j][i]);
         }
     }
 }
@@ -222,7 +231,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_scan_join(ScanArgs a) {
         for (int j = 0; j < kAhead; ++j) {
             if (k + j >= a.chunks - 1) break;
             const int slot = BACK ? a.chunks - 1 - (k + j) : 1 + k + j;
-            h = k + j == 0 ? mine[j] : fmaf(exp2_hw(sum[j] * A2), h, mine[j]);
+            h = k + j == 0 ? mine[j] : carried(sum[j] * A2, h, mine[j]);
             s[slot * per] = h;
         }
     }

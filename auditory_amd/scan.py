@@ -42,7 +42,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, softplus=
                    state_out=None, keep=False):
     """The recurrence h_t = exp(dt A) h_{t-1} + dt B_t u_t with dt = softplus(delta + delta_bias) (softplus=False: the sum
     itself), and y_t = (sum over the states of C_t h_t + D u_t) * silu(z_t) (z=None: no gate), for every channel.  A and the
-    states must be finite.
+    states must be finite, and so must exp(dt A) of every single step.
 
     u, delta, z [items, steps, channels] with contiguous channels; A float32 [channels, states], 1 to 64 states; B, C [items,
     steps, groups, states], a group serving channels / groups neighbouring channels; D, delta_bias float32 [channels].  state

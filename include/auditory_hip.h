@@ -549,7 +549,7 @@ int aud_causal_conv_grad_dev(aud_ctx* ctx, const aud_conv_params* p, const void*
 /* selective scan: u, delta, z [n_items, steps, channels], B, C [n_items, steps, groups, states] (groups and states
  * contiguous; a group's B and C serve channels / groups neighbouring channels), A float32 [channels, states], D and
  * delta_bias float32 [channels] or NULL, z NULL for no gate.  1 <= states <= 64; channels a multiple of groups.
- * A, and the states, must be finite.
+ * A, and the states, must be finite, and so must exp(dt A) of every single step (below 2^128; that of many steps need not be).
  *   dt = softplus(delta + delta_bias) (softplus = 0: without it);  h = exp(dt A) h + dt u B;  y = (sum h C + D u) silu(z)
  * state, state_out float32 [n_items, channels, states]: the state in front of the first frame (NULL: zeros) and behind the
  * last of each item.  steps = 1 is the streaming form: one launch, no workspace. */
