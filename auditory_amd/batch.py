@@ -100,12 +100,22 @@ class BatchProcessor:
         """Group norm with an activation on a feature map [n, PY, PX, ...channels] (the gabor output [n, PY, PX, 2, n_gabor]:
         groups=2 is a group a polarity): every group of neighbouring channels is normalised over the item's positions, then
         weight, bias [channels] and act.  Beside kwta() the other way from the raw maps to activations; for training use
-        auditory_amd.norm, which has the gradients."""
+        auditory_amd.norm, which has the gradients.
+
+        lengths: int32 [n], frames: positions along PX, the time axis, at and behind an item's length do not count and come out
+        as zero, in every band (values outside [0, PX] count as the nearer end).  norm.group_norm itself counts rows, so the
+        maps are laid out frames first for it and back: two copies more."""
         from . import norm
         n, py, px = maps.shape[:3]
-        flat = maps.reshape(n, py * px, int(np.prod(maps.shape[3:])))
-        got = norm.group_norm(flat, groups, weight, bias, eps, act, lengths, want_stats=want_stats)
-        return (got[0].view(maps.shape), got[1]) if want_stats else got.view(maps.shape)
+        ch = int(np.prod(maps.shape[3:]))
+        if lengths is None:
+            rows, counts = maps.reshape(n, py * px, ch), None
+        else:
+            rows, counts = maps.transpose(1, 2).reshape(n, px * py, ch), lengths.clamp(0, px) * py
+        y = norm.group_norm(rows, groups, weight, bias, eps, act, counts, want_stats=want_stats)
+        y, stats = y if want_stats else (y, None)
+        y = y.view(maps.shape) if lengths is None else y.view(n, px, py, *maps.shape[3:]).transpose(1, 2).contiguous()
+        return (y, stats) if want_stats else y
 
     def process_norm(self, sig, items_dev, n_items, pools_y, pools_x, groups, weight=None, bias=None, eps=1e-5, act="relu"):
         """ProcessSegment + ApplyGabor + group norm with an activation for every item, device-resident end to end:
