@@ -1,5 +1,7 @@
 // C ABI, host-staged entry points: the reference's per-step and per-segment calls on caller-owned host buffers, staged
 // through the context's workspaces and stream (HostCallGuard).  See include/auditory_hip.h.
+#include <cstdio>
+
 #include "capi_internal.h"
 
 using namespace audc;
@@ -7,6 +9,27 @@ using namespace audc;
 extern "C" {
 
 namespace {
+
+// all of [p, p + bytes) is memory of this process that it may read and write
+bool mapped_for_writing(const void* p, int64_t bytes) {
+    std::FILE* f = std::fopen("/proc/self/maps", "r");
+    if (!f) return false;
+    uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    const uintptr_t end = at + uintptr_t(bytes);
+    char line[512];
+    bool start = true;  // (a path can be longer than the buffer: what follows is no line of its own)
+    while (at < end && std::fgets(line, sizeof(line), f)) {
+        unsigned long lo = 0, hi = 0;
+        char mode[5] = "";
+        if (start && std::sscanf(line, "%lx-%lx %4s", &lo, &hi, mode) == 3 && hi > at) {
+            if (lo > at || mode[0] != 'r' || mode[1] != 'w') break;  // (the ranges come in order)
+            at = hi;
+        }
+        start = std::strchr(line, '\n') != nullptr;
+    }
+    std::fclose(f);
+    return at >= end;
+}
 
 int check_items(aud_ctx* c, const aud_item* items, int n_items, int64_t sig_total) {
     for (int i = 0; i < n_items; ++i)
@@ -118,10 +141,12 @@ int aud_host_register(aud_ctx* c, void* ptr, int64_t bytes) {
                 return fail(c, AUD_EINVAL, "aud_host_register: the range overlaps a block the context already holds");
     }
     void* dev = nullptr;
-    if (hipHostRegister(ptr, size_t(bytes), hipHostRegisterPortable | hipHostRegisterMapped) != hipSuccess) {
-        // (some machines refuse it for memory that exists already: the range is noted without a device address, and results in
-        // it take the staging route)
+    if (const hipError_t e = hipHostRegister(ptr, size_t(bytes), hipHostRegisterPortable | hipHostRegisterMapped)) {
         (void)hipGetLastError();
+        // some machines refuse it for memory that exists already, with hipErrorInvalidValue: the range is noted without a device
+        // address, and results in it take the staging route.  The same status says that a range is not there or cannot be
+        // written, which is the caller's mistake, as is every other one
+        if (e != hipErrorInvalidValue || !mapped_for_writing(ptr, bytes)) return hip_fail(c, e, "aud_host_register");
         c->host_blocks.push_back({static_cast<unsigned char*>(ptr), size_t(bytes), nullptr, true});
         return AUD_OK;
     }

@@ -351,8 +351,9 @@ int aud_host_free(aud_ctx* ctx, void* ptr);
  * (POSIX shared memory): one process per GPU, each registering the mapping and passing its shard's slice of one
  * [B, ...] float64 tensor as the output of its _host / _sig calls -- the features of the whole batch end in one host tensor
  * with no collective and no copy on the host (the host mode of the reference's multi-GPU use: sound/sndenv.go has no
- * counterpart).  Where the runtime refuses to register memory that exists already, the range is only
- * noted: results in it take the staging route, with the same values.  aud_host_unregister before unmapping; aud_shutdown
+ * counterpart).  Where the runtime refuses to register memory that exists already (hipErrorInvalidValue
+ * for a range that is mapped and writable), the range is only noted: results in it take the staging route, with the same
+ * values; any other failure is AUD_EHIP.  aud_host_unregister before unmapping; aud_shutdown
  * unregisters what is left. */
 int aud_host_register(aud_ctx* ctx, void* ptr, int64_t bytes);
 int aud_host_unregister(aud_ctx* ctx, void* ptr);

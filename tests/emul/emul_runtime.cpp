@@ -22,6 +22,9 @@
 #include <vector>
 
 thread_local dim3 threadIdx, blockIdx, blockDim, gridDim;
+extern "C" {
+int aud_emul_host_register_status = 0;
+}
 
 namespace aud {
 // the one dynamic-LDS allocation of the running workgroup (160 KiB per CU on MI355X)

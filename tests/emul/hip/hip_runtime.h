@@ -174,7 +174,8 @@ enum { hipHostMallocDefault = 0 };
 inline hipError_t hipHostMalloc(void** p, size_t bytes, unsigned) { return hipMalloc(p, bytes); }
 inline hipError_t hipHostFree(void* p) { return hipFree(p); }
 enum { hipHostRegisterPortable = 1, hipHostRegisterMapped = 2 };
-inline hipError_t hipHostRegister(void*, size_t, unsigned) { return hipSuccess; }
+extern "C" int aud_emul_host_register_status;  // what hipHostRegister returns (tests of its failures set it)
+inline hipError_t hipHostRegister(void*, size_t, unsigned) { return aud_emul_host_register_status; }
 inline hipError_t hipHostUnregister(void*) { return hipSuccess; }
 inline hipError_t hipHostGetDevicePointer(void** dev, void* host, unsigned) {
     *dev = host;
