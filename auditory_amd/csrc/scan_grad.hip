@@ -129,16 +129,17 @@ __global__ void __launch_bounds__(64 * W, 2) k_scan_grad(ScanArgs a, int blocks)
     // addresses of this thread's channels in its row of the tile, moved back by 16 rows a tile (rows behind the last one: the last)
     typedef typename Elem<DT>::raw raw;
     const int cc = c < at.dn ? c : 0, left = at.dn - cc;
+    const bool any = first < end;  // (no frame at all: the buffers may be null, nothing is pointed at)
     const int64_t row = (end - 1) * kT + pt, over = row < a.L ? 0 : row - (a.L - 1);
-    const raw* pu = static_cast<const raw*>(a.u) + u0 + (row - over) * a.ur + cc;
-    const raw* pd = static_cast<const raw*>(a.delta) + e0 + (row - over) * a.er + cc;
-    const raw* pg = static_cast<const raw*>(a.dy) + g0 + (row - over) * a.yr + cc;
-    const raw* pz = a.z ? static_cast<const raw*>(a.z) + z0 + (row - over) * a.zr + cc : pg;  // (no gate: read and not used)
+    const raw* pu = any ? static_cast<const raw*>(a.u) + u0 + (row - over) * a.ur + cc : nullptr;
+    const raw* pd = any ? static_cast<const raw*>(a.delta) + e0 + (row - over) * a.er + cc : nullptr;
+    const raw* pg = any ? static_cast<const raw*>(a.dy) + g0 + (row - over) * a.yr + cc : nullptr;
+    const raw* pz = a.z && any ? static_cast<const raw*>(a.z) + z0 + (row - over) * a.zr + cc : pg;  // (no gate: read and not used)
     const int64_t su = kT * a.ur, sd = kT * a.er, sg = kT * a.yr, sz = a.z ? kT * a.zr : sg;
     const int64_t step_o = int64_t(kT) * a.Dn;
     const int lane_in = live ? lane : 0;
     // (the same for all lanes: states in front of the tile, results of its first row)
-    const float* pk = PASS == 3 ? a.kept + ((int64_t(at.b) * tiles + (end - 1)) * a.N + wave * NW) * a.Dn + at.d0 : nullptr;
+    const float* pk = PASS == 3 && any ? a.kept + ((int64_t(at.b) * tiles + (end - 1)) * a.N + wave * NW) * a.Dn + at.d0 : nullptr;
     const unsigned lane_o = unsigned((int64_t(pt) * a.Dn + c) * int(sizeof(raw)));  // bytes: 16 rows of 2^24 channels at most
     int64_t o_tile = o0 + int64_t(end - 1) * step_o;
     const int64_t gn = int64_t(a.G) * a.N, table_bc = int64_t(a.B) * a.L * gn;
@@ -157,11 +158,12 @@ __global__ void __launch_bounds__(64 * W, 2) k_scan_grad(ScanArgs a, int blocks)
                 if (wave * NW + i < a.N) h0[i] = pk[int64_t(i) * a.Dn + lane_in];
     };
     wait_loads();
-    if (first < end) {
+    if (any) {
         fetch();
         pu += over * a.ur, pd += over * a.er, pg += over * a.yr, pz += over * (a.z ? a.zr : a.yr);
     }
-    ScalarTable bc = (ScalarTable)(a.table + ((int64_t(at.b) * a.G + at.g) * tiles + (end - 1)) * kT * 2 * NP + wave * kT * 2 * NW);
+    ScalarTable bc =
+        (ScalarTable)(any ? a.table + ((int64_t(at.b) * a.G + at.g) * tiles + (end - 1)) * kT * 2 * NP + wave * kT * 2 * NW : nullptr);
     for (int tile = end - 1; tile >= first; --tile, bc -= kT * 2 * NP) {
         const int t0 = tile * kT, t = t0 + pt;
         const bool on = t < len;

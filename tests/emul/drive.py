@@ -15,8 +15,35 @@ from auditory_amd import capi  # noqa: E402
 from oracle import oracle as orc  # noqa: E402
 
 
+def frames_cases(lib, variant):
+    """group norm, causal convolution and selective scan: every route, sweeps that do not fit the workgroup, odd widths, lengths
+    (ThreadSanitizer, under which a workgroup's barrier takes milliseconds: one of each kernel)"""
+    import torch
+    import frame_cases as F
+    import norm_cases as N
+    from auditory_amd import frames, runtime
+    torch.set_num_threads(1)
+    native = frames.native()
+    frames.context = lambda x, name: runtime.get_ctx(0).handle.value
+    frames.bind(native, lib, False)
+    wide = [c for c in N.WIDE if c[:3] in ((2, 6, 257), (2, 40, 257), (2, 40, 301), (2, 6, 513), (1, 3, 2052), (1, 7, 2056), (2, 9, 1540))]
+    runs = [(N.case, c) for c in wide + N.ROUTES[:3]] + [(F.norm_case, c) for c in F.NORM[:4]]
+    runs += [(F.conv_case, c) for c in F.CONV] + [(F.scan_case, c) for c in F.SCAN]
+    if variant == "tsan":
+        runs = [(N.case, (1, 3, 24, 3, "f32", "silu", True, None, 0)), (N.case, (1, 130, 65, 5, "f32", "silu", True, None, 0)),
+                (F.conv_case, F.CONV[3]), (F.scan_case, F.SCAN[1]), (F.scan_case, (1, 130, 4, 1, 4, "f32", True, True, True, True, True, None, 0))]
+    for fn, c in runs:
+        print(fn.__name__, c, flush=True)
+        fn("cpu", *c)
+
+
 def main():
     variant, which = sys.argv[1], sys.argv[2]
+    if which == "frames":
+        with backend.emulated(variant) as lib:
+            frames_cases(lib, variant)
+        print("DRIVE-OK", variant, which)
+        return
     by_name = {c[0]: c for c in PC.CASES}
     with backend.emulated(variant):
         if which == "quick":
