@@ -45,6 +45,17 @@ std::string shape_text(Shape s) {
     return t + "]";
 }
 
+// Nothing here is recorded for autograd: a tensor that asks for gradients, in a call that autograd would have to record, would
+// lose them without a word.
+bool asks(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
+bool asks(const Maybe& t) { return t && asks(*t); }
+template <typename... T>
+void no_autograd(const T&... tensors) {
+    if (at::GradMode::is_enabled() && (asks(tensors) || ...))
+        bad("a tensor of this call requires grad, and the call records nothing for autograd: make it within torch.no_grad() or in "
+            "the forward or backward of an autograd.Function (the gradients are a call of their own)");
+}
+
 // one call: the tensor that sets type and device, the context
 struct Call {
     const at::Tensor& x;
@@ -127,6 +138,7 @@ aud_norm_params norm_params(const Call& c, int64_t groups, int act, double eps) 
 }
 std::tuple<at::Tensor, Maybe> group_norm(uintptr_t ctx, const at::Tensor& x, int64_t groups, const Maybe& weight, const Maybe& bias, double eps,
                                          int act, const Maybe& lengths, const Maybe& out, Maybe stats, bool want_stats) {
+    no_autograd(x, weight, bias, out, stats);
     const Call c(x, ctx, "x", 3, 3);
     const aud_norm_params p = norm_params(c, groups, act, eps);
     const at::Tensor y = c.out(out);
@@ -141,6 +153,7 @@ std::tuple<at::Tensor, Maybe> group_norm(uintptr_t ctx, const at::Tensor& x, int
 std::tuple<at::Tensor, Maybe, Maybe> group_norm_grad(uintptr_t ctx, const at::Tensor& dy, const at::Tensor& x, const at::Tensor& stats,
                                                      int64_t groups, const Maybe& weight, const Maybe& bias, double eps, int act,
                                                      const Maybe& lengths, const Maybe& out) {
+    no_autograd(dy, x, stats, weight, bias, out);
     const Call c(x, ctx, "x", 3, 3);
     aud_norm_params p = norm_params(c, groups, act, eps);
     c.rows(dy, "dy", x.sizes(), 1, &p.dy_item, &p.dy_row);
@@ -171,6 +184,7 @@ aud_conv_params conv_params(const Call& c, const at::Tensor& weight, int act) {
 }
 at::Tensor causal_conv(uintptr_t ctx, bool one_frame, const at::Tensor& x, const at::Tensor& weight, const Maybe& bias, int act, const Maybe& state,
                        const Maybe& lengths, const Maybe& out, const Maybe& state_out) {
+    no_autograd(x, weight, bias, state, out, state_out);
     const int axes = one_frame ? 2 : 3;
     const Call c(x, ctx, "x", axes, axes);
     const aud_conv_params p = conv_params(c, weight, act);
@@ -183,6 +197,7 @@ at::Tensor causal_conv(uintptr_t ctx, bool one_frame, const at::Tensor& x, const
 std::tuple<at::Tensor, at::Tensor, Maybe, Maybe> causal_conv_grad(uintptr_t ctx, const at::Tensor& dy, const at::Tensor& x, const at::Tensor& weight,
                                                                   const Maybe& bias, int act, const Maybe& state, const Maybe& lengths,
                                                                   const Maybe& dstate_out, const Maybe& out) {
+    no_autograd(dy, x, weight, bias, state, dstate_out, out);
     const Call c(x, ctx, "x", 3, 3);
     aud_conv_params p = conv_params(c, weight, act);
     c.rows(dy, "dy", x.sizes(), 1, &p.dy_item, &p.dy_row);
@@ -244,6 +259,7 @@ std::tuple<at::Tensor, Maybe> selective_scan(uintptr_t ctx, bool one_frame, cons
                                              const at::Tensor& B, const at::Tensor& C, const Maybe& D, const Maybe& z, const Maybe& delta_bias,
                                              bool softplus, const Maybe& state, const Maybe& lengths, const Maybe& out, const Maybe& state_out,
                                              bool keep) {
+    no_autograd(u, delta, A, B, C, D, z, delta_bias, state, out, state_out);
     const Scan s(ctx, one_frame ? 2 : 3, u, delta, A, B, C, z, softplus);
     const at::Tensor y = s.c.out(out);
     at::Tensor kept;
@@ -258,6 +274,7 @@ std::tuple<at::Tensor, Maybe> selective_scan(uintptr_t ctx, bool one_frame, cons
 py::tuple selective_scan_grad(uintptr_t ctx, const at::Tensor& dy, const at::Tensor& u, const at::Tensor& delta, const at::Tensor& A,
                               const at::Tensor& B, const at::Tensor& C, const at::Tensor& kept, const Maybe& D, const Maybe& z,
                               const Maybe& delta_bias, bool softplus, const Maybe& state, const Maybe& lengths, const Maybe& dstate_out) {
+    no_autograd(dy, u, delta, A, B, C, kept, D, z, delta_bias, state, dstate_out);
     Scan s(ctx, 3, u, delta, A, B, C, z, softplus);
     const Call& c = s.c;
     c.rows(dy, "dy", u.sizes(), 1, &s.p.dy_item, &s.p.dy_row);

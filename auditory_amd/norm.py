@@ -2,7 +2,8 @@
 [n_items, PY * PX, 2 * n_gabor], mel frames [n_items, T, nf], or whatever a network made of them.
 
 Device-resident, on torch's current stream; float32, bfloat16 or float16 maps with float32 parameters.  The gradients are
-functions of their own: nothing here records for torch's autograd."""
+functions of their own: nothing here records for torch's autograd, so a tensor that requires grad is refused while autograd
+records -- use torch.no_grad(), or an autograd.Function whose backward is the gradients' call."""
 from . import frames
 
 _ACTS = ("none", "relu", "silu", "gelu")

@@ -3,7 +3,8 @@ the selective state space scan (aud_scan_*, scan.hip), for whole utterances, wit
 with the state carried between calls.
 
 Device-resident, on torch's current stream; float32, bfloat16 or float16 frames with float32 parameters and scan states.  The
-gradients are functions of their own: nothing here records for torch's autograd."""
+gradients are functions of their own: nothing here records for torch's autograd, so a tensor that requires grad is refused
+while autograd records -- use torch.no_grad(), or an autograd.Function whose backward is the gradients' call."""
 from collections import namedtuple
 
 from . import frames

@@ -5,7 +5,7 @@ import torch
 
 import frame_cases as F
 import frame_ref as R
-from auditory_amd import scan
+from auditory_amd import capi, norm, scan
 from test_norm_widths import emu, emu_lib  # noqa: F401  (fixtures)
 
 gpu = pytest.mark.gpu
@@ -83,3 +83,91 @@ def test_emul_decays_past_float32_many_chunks(emu):  # noqa: F811
 @gpu
 def test_gpu_decays_past_float32_many_chunks():
     many_chunks("cuda:0")
+
+
+# ---- inputs that ask for gradients -------------------------------------------------------------------------------------------
+
+def calls(dev):
+    """(name, call, its tensors by argument) of every entry point"""
+    m = F.Make(dev, 13, "f32")
+    x, dy, w, b = m.n(2, 5, 8), m.n(2, 5, 8), m.n(8), m.n(8)
+    _, st = norm.group_norm(x, 2, w, b, want_stats=True)
+    cw, cs = m.n(8, 3), m.n(2, 2, 8)
+    a = F.scan_inputs(m, 2, 5, 8, 1, 4, True, True, True, True, True)
+    one = {n: a[n][:, 0] if n in ("u", "delta", "B", "C", "z") else a[n] for n in a}
+    _, kept = scan.selective_scan(**a, softplus=True, keep=True)
+    return [
+        ("group_norm", lambda **t: norm.group_norm(groups=2, **t), dict(x=x, weight=w, bias=b)),
+        ("group_norm_grad", lambda **t: norm.group_norm_grad(groups=2, **t), dict(dy=dy, x=x, stats=st, weight=w, bias=b)),
+        ("causal_conv", lambda **t: scan.causal_conv(**t), dict(x=x, weight=cw, bias=b, state=cs)),
+        ("causal_conv_step", lambda **t: scan.causal_conv_step(**t), dict(x=x[:, 0], state=cs.clone(), weight=cw, bias=b)),
+        ("causal_conv_grad", lambda **t: scan.causal_conv_grad(**t), dict(dy=dy, x=x, weight=cw, bias=b, state=cs, dstate_out=cs)),
+        ("selective_scan", lambda **t: scan.selective_scan(softplus=True, **t), a),
+        ("selective_scan_step", lambda **t: scan.selective_scan_step(softplus=True, **t), {**one, "state": one["state"].clone()}),
+        ("selective_scan_grad", lambda **t: scan.selective_scan_grad(softplus=True, **t), dict(a, dy=dy, kept=kept, dstate_out=a["state"])),
+    ]
+
+
+def flat(out):
+    return [t for t in (out if isinstance(out, tuple) else (out,)) if t is not None]
+
+
+def gradients_asked_for(dev):
+    """nothing is recorded for autograd, so a call that autograd would have to record is refused; within no_grad (and so in the
+    forward and backward of an autograd.Function) the same tensors are taken"""
+    for name, call, tensors in calls(dev):
+        fresh = lambda: {n: t.clone() for n, t in tensors.items()}  # noqa: E731
+        want = flat(call(**fresh()))
+        for n in tensors:
+            asks = fresh()
+            asks[n].requires_grad_(True)
+            with pytest.raises(capi.AuditoryError) as e:
+                call(**asks)
+            assert e.value.status == capi.AUD_EINVAL and "no_grad" in str(e.value), (name, n)
+            with torch.no_grad():
+                got = flat(call(**asks))
+            assert all(torch.equal(p, q) and not p.requires_grad for p, q in zip(got, want)), (name, n)
+    with pytest.raises(capi.AuditoryError):
+        x = torch.zeros(2, 5, 8, device=dev)
+        norm.group_norm(x, 2, out=torch.zeros_like(x).requires_grad_(True))
+
+
+def test_emul_gradients_asked_for(emu):  # noqa: F811
+    gradients_asked_for("cpu")
+
+
+@gpu
+def test_gpu_gradients_asked_for():
+    gradients_asked_for("cuda:0")
+
+
+class Normed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b):
+        y, stats = norm.group_norm(x, 2, w, b, act="silu", want_stats=True)
+        ctx.save_for_backward(x, w, b, stats)
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w, b, stats = ctx.saved_tensors
+        return norm.group_norm_grad(dy.contiguous(), x, stats, 2, w, b, act="silu")
+
+
+def in_a_function(dev):
+    m = F.Make(dev, 17, "f32")
+    x, dy, w, b = m.n(2, 5, 8), m.n(2, 5, 8), m.n(8), m.n(8)
+    _, st = norm.group_norm(x, 2, w, b, act="silu", want_stats=True)
+    want = norm.group_norm_grad(dy, x, st, 2, w, b, act="silu")
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    (Normed.apply(*leaves) * dy).sum().backward()
+    assert all(torch.equal(t.grad, q) for t, q in zip(leaves, want))
+
+
+def test_emul_in_a_function(emu):  # noqa: F811
+    in_a_function("cpu")
+
+
+@gpu
+def test_gpu_in_a_function():
+    in_a_function("cuda:0")
