@@ -20,7 +20,7 @@ struct Run {  // the run of steps and the pack of channels of this thread
     int c, t0, t1, tile;
     bool on;
     __device__ __forceinline__ Run(const ConvArgs& a, int V, int tiles) {
-        const int64_t id = int64_t(blockIdx.x) * kNT + threadIdx.x;
+        const int64_t id = int64_t(a.first + blockIdx.x) * kNT + threadIdx.x;
         const int packs = a.D / V;
         const int64_t q = id / packs;
         c = int(id % packs) * V;
@@ -222,13 +222,15 @@ template <int DT, int V, int K, int ACT>
 hipError_t run(const ConvArgs& a, bool grad, hipStream_t st) {
     const int tiles = tiles_of(a);
     const int64_t threads = int64_t(a.B) * tiles * (a.D / V);
-    const dim3 grid(unsigned((threads + kNT - 1) / kNT));
-    if (!grad) {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv<DT, V, K, ACT>), grid, dim3(kNT), 0, st, a, tiles);
-        return hipGetLastError();
-    }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_grad<DT, V, K, ACT>), grid, dim3(kNT), 0, st, a, tiles);
-    if (hipError_t e = hipGetLastError()) return e;
+    const int64_t blocks = (threads + kNT - 1) / kNT;
+    if (!grad)
+        return in_slices_of(a, blocks, kNT, [&](dim3 grid, const ConvArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv<DT, V, K, ACT>), grid, dim3(kNT), 0, st, s, tiles);
+        });
+    if (hipError_t e = in_slices_of(a, blocks, kNT, [&](dim3 grid, const ConvArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_conv_grad<DT, V, K, ACT>), grid, dim3(kNT), 0, st, s, tiles);
+        }))
+        return e;
     if (!a.dweight && !a.dbias) return hipSuccess;
     return launch_column_sums(a.part, int64_t(a.B) * tiles, a.D, K, 1, a.dweight, a.dbias, nullptr, st);
 }

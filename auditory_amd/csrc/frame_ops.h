@@ -109,6 +109,31 @@ hipError_t allow_lds(size_t bytes) {
     return e;
 }
 
+// A launch holds fewer than 2^32 threads.  A grid of more goes out in slices, in order on the stream: launch(grid, first) for the
+// workgroups from `first` on.  What a slice's launch refuses ends the call; nothing is queued behind it.  (The CPU emulator is built
+// with a small limit, so that slices are what its tests run.)
+#ifndef AUD_LAUNCH_THREADS
+#define AUD_LAUNCH_THREADS 0xFFFFFFFFll
+#endif
+template <typename F>
+hipError_t in_slices(int64_t blocks, int threads, F&& launch) {
+    const int64_t most = int64_t(AUD_LAUNCH_THREADS) / threads;
+    for (int64_t first = 0; first < blocks; first += most) {
+        launch(dim3(unsigned(std::min(most, blocks - first))), unsigned(first));
+        if (hipError_t e = hipGetLastError()) return e;
+    }
+    return hipSuccess;
+}
+// the same for a kernel whose first argument is its descriptor, with the slice's start in it
+template <typename A, typename F>
+hipError_t in_slices_of(const A& a, int64_t blocks, int threads, F&& launch) {
+    return in_slices(blocks, threads, [&](dim3 grid, unsigned first) {
+        A s = a;
+        s.first = first;
+        launch(grid, s);
+    });
+}
+
 // rows of an item that count: lengths[b] held to [0, rows]; rows where there is no table
 __device__ __forceinline__ int item_rows(const int32_t* lengths, int b, int rows) {
     if (!lengths) return rows;
@@ -133,6 +158,7 @@ struct NormArgs {
     int64_t xi, xr, di, dr;
     float eps;
     int chunks, chunk_rows;
+    unsigned first;           // workgroups in front of this launch's (in_slices)
 };
 struct NormRoute {
     int vec;                 // elements per access
@@ -160,6 +186,7 @@ struct ConvArgs {
     int B, L, D;
     int64_t xi, xr, di, dr;
     int T;                    // steps a thread walks
+    unsigned first;           // workgroups in front of this launch's
 };
 int conv_tile(int dtype, int B, int L, int D, int align);
 hipError_t launch_conv(const ConvArgs& a, int dtype, int act, int K, int align, hipStream_t st);
@@ -186,6 +213,7 @@ struct ScanArgs {
     int B, L, Dn, G, N, softplus;
     int64_t ui, ur, ei, er, zi, zr, yi, yr, bi, br, ci, cr;  // item / row strides of u, delta, z, dy, Bm, Cm
     int chunks, chunk_tiles, fold;
+    unsigned first;                  // workgroups in front of this launch's
 };
 struct ScanRoute {
     int chunks, chunk_tiles;  // the time axis in `chunks` runs of chunk_tiles tiles, scanned side by side and joined

@@ -197,7 +197,7 @@ __device__ __forceinline__ void apply_rows(const NormArgs& a, int b, int lo, int
 template <int DT, int V, int ACT>
 __global__ void __launch_bounds__(kItemThreads) k_norm_item(NormArgs a) {
     float* stats = reinterpret_cast<float*>(dyn_lds());  // [G, 2]
-    const int b = blockIdx.x, rows = item_rows(a.lengths, b, a.S);
+    const int b = a.first + blockIdx.x, rows = item_rows(a.lengths, b, a.S);
     group_moments<DT, V, kItemThreads>(a, b, 0, rows, stats + 2 * a.G, stats);
     for (int g = threadIdx.x; g < a.G; g += kItemThreads) {
         const float r = inv_std(stats[2 * g + 1], rows, a.C / a.G, a.eps);
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kItemThreads) k_norm_held(NormArgs a) {
     constexpr int NT = kItemThreads, R = 4;
     float* stats = reinterpret_cast<float*>(dyn_lds());  // [G, 2]
     float* entries = stats + 2 * a.G;                    // [lanes][C]
-    const int b = blockIdx.x, rows = item_rows(a.lengths, b, a.S), packs = a.C / V, cg = a.C / a.G;
+    const int b = a.first + blockIdx.x, rows = item_rows(a.lengths, b, a.S), packs = a.C / V, cg = a.C / a.G;
     const Lanes<NT, false> l(packs, 0);
     const bool mine = l.r < l.lanes;
     const int64_t base = int64_t(b) * a.xi + int64_t(l.c) * V;
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(kItemThreads) k_norm_held(NormArgs a) {
 template <int DT, int V>
 __global__ void __launch_bounds__(kChunkThreads) k_norm_chunk(NormArgs a) {
     float* moments = reinterpret_cast<float*>(dyn_lds());
-    const int chunk = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks, rows = item_rows(a.lengths, b, a.S);
+    const int chunk = (a.first + blockIdx.x) % a.chunks, b = (a.first + blockIdx.x) / a.chunks, rows = item_rows(a.lengths, b, a.S);
     const int lo = chunk * a.chunk_rows, hi = lo + a.chunk_rows < rows ? lo + a.chunk_rows : rows;
     group_moments<DT, V, kChunkThreads>(a, b, lo, hi, moments + 2 * a.G, moments);
     float* out = a.part + (int64_t(b) * a.chunks + chunk) * a.G * 2;
@@ -350,7 +350,7 @@ __device__ __forceinline__ void join_chunks(const NormArgs& a, int b, int g, int
     r = inv_std(sum_lanes(m2, p), rows, cg, a.eps);
 }
 __global__ void __launch_bounds__(kChunkThreads) k_norm_join(NormArgs a) {  // many groups: a thread each
-    const int64_t i = int64_t(blockIdx.x) * kChunkThreads + threadIdx.x;
+    const int64_t i = int64_t(a.first + blockIdx.x) * kChunkThreads + threadIdx.x;
     if (i >= int64_t(a.B) * a.G) return;
     const int b = int(i / a.G), g = int(i % a.G);
     float m, r;
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kChunkThreads) k_norm_join(NormArgs a) {  // m
 template <int DT, int V, int ACT, bool JOIN>
 __global__ void __launch_bounds__(kChunkThreads) k_norm_apply(NormArgs a) {
     float* stats = reinterpret_cast<float*>(dyn_lds());
-    const int chunk = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks, rows = item_rows(a.lengths, b, a.S);
+    const int chunk = (a.first + blockIdx.x) % a.chunks, b = (a.first + blockIdx.x) / a.chunks, rows = item_rows(a.lengths, b, a.S);
     const int lo = chunk * a.chunk_rows, hi = lo + a.chunk_rows < a.S ? lo + a.chunk_rows : a.S;
     if constexpr (JOIN) {
         for_groups<kChunkThreads>(a.G, [&](int g, int lane, int p, bool there) {
@@ -503,7 +503,7 @@ template <int DT, int V, int ACT>
 __global__ void __launch_bounds__(kItemThreads) k_norm_grad_item(NormArgs a) {
     float* stats = reinterpret_cast<float*>(dyn_lds());  // [G, 2]
     float *gsum = stats + 2 * a.G, *sums = gsum + 2 * a.G, *entries = sums + 2 * a.C;
-    const int b = blockIdx.x, rows = item_rows(a.lengths, b, a.S);
+    const int b = a.first + blockIdx.x, rows = item_rows(a.lengths, b, a.S);
     for (int i = threadIdx.x; i < 2 * a.G; i += kItemThreads) stats[i] = a.stats[int64_t(b) * a.G * 2 + i];
     __syncthreads();
     channel_sums<DT, V, ACT, kItemThreads>(a, b, 0, rows, stats, entries, sums);
@@ -521,7 +521,7 @@ template <int DT, int V, int ACT>
 __global__ void __launch_bounds__(kChunkThreads) k_norm_grad_chunk(NormArgs a) {
     float* stats = reinterpret_cast<float*>(dyn_lds());
     float *sums = stats + 2 * a.G, *entries = sums + 2 * a.C;
-    const int chunk = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks, rows = item_rows(a.lengths, b, a.S);
+    const int chunk = (a.first + blockIdx.x) % a.chunks, b = (a.first + blockIdx.x) / a.chunks, rows = item_rows(a.lengths, b, a.S);
     const int lo = chunk * a.chunk_rows, hi = lo + a.chunk_rows < rows ? lo + a.chunk_rows : rows;
     for (int i = threadIdx.x; i < 2 * a.G; i += kChunkThreads) stats[i] = a.stats[int64_t(b) * a.G * 2 + i];
     __syncthreads();
@@ -533,8 +533,8 @@ __global__ void __launch_bounds__(kChunkThreads) k_norm_grad_chunk(NormArgs a) {
 constexpr int kJoinCols = 64, kJoinLanes = 4;
 __global__ void __launch_bounds__(kJoinCols * kJoinLanes) k_norm_grad_join(NormArgs a) {
     float* lds = reinterpret_cast<float*>(dyn_lds());
-    const int blocks = (2 * a.C + kJoinCols - 1) / kJoinCols, b = blockIdx.x / blocks;
-    const int c = blockIdx.x % blocks * kJoinCols + threadIdx.x % kJoinCols, lane = threadIdx.x / kJoinCols;
+    const int blocks = (2 * a.C + kJoinCols - 1) / kJoinCols, b = (a.first + blockIdx.x) / blocks;
+    const int c = (a.first + blockIdx.x) % blocks * kJoinCols + threadIdx.x % kJoinCols, lane = threadIdx.x / kJoinCols;
     float s = 0.f;
     if (c < 2 * a.C)
 #pragma unroll 4
@@ -551,8 +551,8 @@ template <int DT, int V, int ACT>
 __global__ void __launch_bounds__(kChunkThreads) k_norm_grad_apply(NormArgs a) {
     const float* sums = a.part + int64_t(a.B) * a.chunks * 2 * a.C;
     const int64_t work = int64_t(a.B) * a.chunks;
-    if (blockIdx.x >= work) {
-        const int c = int(blockIdx.x - work) * kChunkThreads + int(threadIdx.x);
+    if (a.first + blockIdx.x >= work) {
+        const int c = int(a.first + blockIdx.x - work) * kChunkThreads + int(threadIdx.x);
         if (c >= 2 * a.C) return;
         float s = 0.f;
 #pragma unroll 8
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kChunkThreads) k_norm_grad_apply(NormArgs a) {
     }
     float* stats = reinterpret_cast<float*>(dyn_lds());
     float* gsum = stats + 2 * a.G;
-    const int chunk = blockIdx.x % a.chunks, b = blockIdx.x / a.chunks, rows = item_rows(a.lengths, b, a.S);
+    const int chunk = (a.first + blockIdx.x) % a.chunks, b = (a.first + blockIdx.x) / a.chunks, rows = item_rows(a.lengths, b, a.S);
     const int lo = chunk * a.chunk_rows, hi = lo + a.chunk_rows < a.S ? lo + a.chunk_rows : a.S;
     for (int i = threadIdx.x; i < 2 * a.G; i += kChunkThreads) stats[i] = a.stats[int64_t(b) * a.G * 2 + i];
     group_sums<kChunkThreads>(a, rows, sums + int64_t(b) * 2 * a.C, gsum);
@@ -573,10 +573,10 @@ __global__ void __launch_bounds__(kChunkThreads) k_norm_grad_apply(NormArgs a) {
 // ---- column sums of a partial-result table ------------------------------------------------------------------------------
 constexpr int kCsCols = 32, kCsLanes = 32;
 __global__ void __launch_bounds__(kCsCols * kCsLanes) k_column_sums(const float* in, int64_t rows, int W, int K, int extra, float* out0,
-                                                                   float* out1, float* out2) {
+                                                                   float* out1, float* out2, unsigned first) {
     float* lds = reinterpret_cast<float*>(dyn_lds());
     const int c = threadIdx.x % kCsCols, lane = threadIdx.x / kCsCols;
-    const int64_t width = int64_t(W) * (K + extra), col = int64_t(blockIdx.x) * kCsCols + c;
+    const int64_t width = int64_t(W) * (K + extra), col = int64_t(first + blockIdx.x) * kCsCols + c;
     float s = 0.f;
     if (col < width)
 #pragma unroll 4
@@ -607,27 +607,36 @@ hipError_t run(const NormArgs& a, const NormRoute& r, hipStream_t st) {
     if (r.one_wg && packs <= kItemThreads && int64_t(a.S) <= 4 * (kItemThreads / packs)) {
         const size_t lds = (2 * size_t(a.G) + size_t(kItemThreads / packs) * a.C) * 4;
         if (hipError_t e = allow_lds<&k_norm_held<DT, V, ACT>>(lds)) return e;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_held<DT, V, ACT>), dim3(unsigned(a.B)), dim3(kItemThreads), lds, st, a);
-        return hipGetLastError();
+        return in_slices_of(a, a.B, kItemThreads, [&](dim3 grid, const NormArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_held<DT, V, ACT>), grid, dim3(kItemThreads), lds, st, s);
+        });
     }
     if (r.one_wg) {
         const size_t lds = (2 * size_t(a.G) + entries_of(kItemThreads, V, a.C)) * 4;
         if (hipError_t e = allow_lds<&k_norm_item<DT, V, ACT>>(lds)) return e;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_item<DT, V, ACT>), dim3(unsigned(a.B)), dim3(kItemThreads), lds, st, a);
-        return hipGetLastError();
+        return in_slices_of(a, a.B, kItemThreads, [&](dim3 grid, const NormArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_item<DT, V, ACT>), grid, dim3(kItemThreads), lds, st, s);
+        });
     }
-    const dim3 grid(unsigned(a.chunks) * unsigned(a.B)), wg(kChunkThreads);
+    const int64_t work = int64_t(a.chunks) * a.B;
+    const dim3 wg(kChunkThreads);
     const size_t lds = (2 * size_t(a.G) + entries_of(kChunkThreads, V, a.C)) * 4;
     if (hipError_t e = allow_lds<&k_norm_chunk<DT, V>>(lds)) return e;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_chunk<DT, V>), grid, wg, lds, st, a);
-    if (r.join) {
-        const unsigned join = unsigned((int64_t(a.B) * a.G + kChunkThreads - 1) / kChunkThreads);
-        hipLaunchKernelGGL(k_norm_join, dim3(join), wg, 0, st, a);
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_apply<DT, V, ACT, false>), grid, wg, size_t(a.G) * 8, st, a);
-    } else {
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_apply<DT, V, ACT, true>), grid, wg, size_t(a.G) * 8, st, a);
-    }
-    return hipGetLastError();
+    if (hipError_t e = in_slices_of(a, work, kChunkThreads, [&](dim3 grid, const NormArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_chunk<DT, V>), grid, wg, lds, st, s);
+        }))
+        return e;
+    if (!r.join)
+        return in_slices_of(a, work, kChunkThreads, [&](dim3 grid, const NormArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_apply<DT, V, ACT, true>), grid, wg, size_t(s.G) * 8, st, s);
+        });
+    const int64_t join = (int64_t(a.B) * a.G + kChunkThreads - 1) / kChunkThreads;
+    if (hipError_t e = in_slices_of(a, join, kChunkThreads,
+                                    [&](dim3 grid, const NormArgs& s) { hipLaunchKernelGGL(k_norm_join, grid, wg, 0, st, s); }))
+        return e;
+    return in_slices_of(a, work, kChunkThreads, [&](dim3 grid, const NormArgs& s) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_apply<DT, V, ACT, false>), grid, wg, size_t(s.G) * 8, st, s);
+    });
 }
 
 template <int DT, int V, int ACT>
@@ -635,20 +644,29 @@ hipError_t run_grad(const NormArgs& a, const NormRoute& r, hipStream_t st) {
     if (r.one_wg) {
         const size_t lds = (4 * size_t(a.G) + 2 * size_t(a.C) + entries_of(kItemThreads, V, a.C)) * 4;
         if (hipError_t e = allow_lds<&k_norm_grad_item<DT, V, ACT>>(lds)) return e;
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_grad_item<DT, V, ACT>), dim3(unsigned(a.B)), dim3(kItemThreads), lds, st, a);
-        if (hipError_t e = hipGetLastError()) return e;
+        if (hipError_t e = in_slices_of(a, a.B, kItemThreads, [&](dim3 grid, const NormArgs& s) {
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_grad_item<DT, V, ACT>), grid, dim3(kItemThreads), lds, st, s);
+            }))
+            return e;
         if (a.B == 1 || (!a.dweight && !a.dbias)) return hipSuccess;
         return launch_column_sums(a.part, a.B, a.C, 0, 2, nullptr, a.dweight, a.dbias, st);
     }
-    const unsigned work = unsigned(a.chunks) * unsigned(a.B);
+    const int64_t work = int64_t(a.chunks) * a.B;
     const size_t lds = (2 * size_t(a.G) + 2 * size_t(a.C) + entries_of(kChunkThreads, V, a.C)) * 4;
     if (hipError_t e = allow_lds<&k_norm_grad_chunk<DT, V, ACT>>(lds)) return e;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_grad_chunk<DT, V, ACT>), dim3(work), dim3(kChunkThreads), lds, st, a);
-    const unsigned join = unsigned(a.B) * unsigned((2 * a.C + kJoinCols - 1) / kJoinCols);
-    hipLaunchKernelGGL(k_norm_grad_join, dim3(join), dim3(kJoinCols * kJoinLanes), size_t(kJoinCols) * kJoinLanes * 4, st, a);
-    const unsigned more = a.dweight || a.dbias ? unsigned((2 * a.C + kChunkThreads - 1) / kChunkThreads) : 0;
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_grad_apply<DT, V, ACT>), dim3(work + more), dim3(kChunkThreads), size_t(a.G) * 16, st, a);
-    return hipGetLastError();
+    if (hipError_t e = in_slices_of(a, work, kChunkThreads, [&](dim3 grid, const NormArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_grad_chunk<DT, V, ACT>), grid, dim3(kChunkThreads), lds, st, s);
+        }))
+        return e;
+    const int64_t join = int64_t(a.B) * ((2 * a.C + kJoinCols - 1) / kJoinCols);
+    if (hipError_t e = in_slices_of(a, join, kJoinCols * kJoinLanes, [&](dim3 grid, const NormArgs& s) {
+            hipLaunchKernelGGL(k_norm_grad_join, grid, dim3(kJoinCols * kJoinLanes), size_t(kJoinCols) * kJoinLanes * 4, st, s);
+        }))
+        return e;
+    const int64_t more = a.dweight || a.dbias ? (2 * a.C + kChunkThreads - 1) / kChunkThreads : 0;
+    return in_slices_of(a, work + more, kChunkThreads, [&](dim3 grid, const NormArgs& s) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_norm_grad_apply<DT, V, ACT>), grid, dim3(kChunkThreads), size_t(s.G) * 16, st, s);
+    });
 }
 
 template <int DT, int V>
@@ -683,9 +701,10 @@ hipError_t by_type(const NormArgs& a, const NormRoute& r, int dtype, int act, bo
 
 hipError_t launch_column_sums(const float* in, int64_t rows, int W, int K, int extra, float* out0, float* out1, float* out2, hipStream_t st) {
     const int64_t width = int64_t(W) * (K + extra);
-    hipLaunchKernelGGL(k_column_sums, dim3(unsigned((width + kCsCols - 1) / kCsCols)), dim3(kCsCols * kCsLanes),
-                       size_t(kCsCols) * kCsLanes * 4, st, in, rows, W, K, extra, out0, out1, out2);
-    return hipGetLastError();
+    return in_slices((width + kCsCols - 1) / kCsCols, kCsCols * kCsLanes, [&](dim3 grid, unsigned first) {
+        hipLaunchKernelGGL(k_column_sums, grid, dim3(kCsCols * kCsLanes), size_t(kCsCols) * kCsLanes * 4, st, in, rows, W, K, extra, out0,
+                           out1, out2, first);
+    });
 }
 
 int vector_of(int e, int C, int align) {

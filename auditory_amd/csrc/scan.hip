@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
 // ---- one frame: four lanes a channel, a quarter of its states each ----------------------------------------------------
 template <int DT>
 __global__ void __launch_bounds__(kNT) k_scan_step(ScanArgs a) {
-    const int64_t id = int64_t(blockIdx.x) * kNT + threadIdx.x, ch = id >> 2;
+    const int64_t id = int64_t(a.first + blockIdx.x) * kNT + threadIdx.x, ch = id >> 2;
     const int part = int(id & 3);
     const bool on = ch < int64_t(a.B) * a.Dn;  // (all lanes of a wave reach the exchange below)
     const int64_t b = on ? ch / a.Dn : 0;
@@ -240,20 +240,22 @@ __global__ void __launch_bounds__(kNT) k_scan_step(ScanArgs a) {
 
 template <int DT, int NW, int W, bool VEC>
 hipError_t run(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
-    const dim3 grid(unsigned(int64_t(a.B) * a.chunks * a.G * r.blocks)), wg(64 * W);
+    const int64_t side = int64_t(a.B) * a.G * r.blocks;  // workgroups side by side in a chunk
+    const dim3 wg(64 * W);
     const size_t lds1 = size_t(4) * kT * kCh * 4, lds3 = lds1 + size_t(2) * W * kT * kCh * 4;
     if (hipError_t e = allow_lds<&k_scan<DT, NW, W, VEC, 3>>(lds3)) return e;
-    run_table<DT>(a, NW * W, NW, st);
+    if (hipError_t e = run_table<DT>(a, NW * W, NW, st)) return e;
     if (a.chunks > 1) {
-        const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 1>), first, wg, lds1, st, a, r.blocks);
-        if (!a.fold) {
-            const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<false>), dim3(join), dim3(kJoinThreads), 0, st, a);
-        }
+        if (hipError_t e = in_slices_of(a, side * (a.chunks - 1), 64 * W, [&](dim3 grid, const ScanArgs& s) {
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 1>), grid, wg, lds1, st, s, r.blocks);
+            }))
+            return e;
+        if (!a.fold)
+            if (hipError_t e = run_join<false>(a, st)) return e;
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 3>), grid, wg, lds3, st, a, r.blocks);
-    return hipGetLastError();
+    return in_slices_of(a, side * a.chunks, 64 * W, [&](dim3 grid, const ScanArgs& s) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan<DT, NW, W, VEC, 3>), grid, wg, lds3, st, s, r.blocks);
+    });
 }
 template <int DT, bool VEC>
 hipError_t by_states(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
@@ -303,13 +305,13 @@ hipError_t launch_scan(const ScanArgs& a, const ScanRoute& r, int dtype, bool al
     return by_type(a, r, dtype, aligned, st);
 }
 hipError_t launch_scan_step(const ScanArgs& a, int dtype, hipStream_t st) {
-    const dim3 grid(unsigned((int64_t(a.B) * a.Dn * 4 + kNT - 1) / kNT));
-    switch (dtype) {
-        case AUD_F32: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_step<AUD_F32>), grid, dim3(kNT), 0, st, a); break;
-        case AUD_BF16: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_step<AUD_BF16>), grid, dim3(kNT), 0, st, a); break;
-        default: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_step<AUD_F16>), grid, dim3(kNT), 0, st, a);
-    }
-    return hipGetLastError();
+    return in_slices_of(a, (int64_t(a.B) * a.Dn * 4 + kNT - 1) / kNT, kNT, [&](dim3 grid, const ScanArgs& s) {
+        switch (dtype) {
+            case AUD_F32: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_step<AUD_F32>), grid, dim3(kNT), 0, st, s); break;
+            case AUD_BF16: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_step<AUD_BF16>), grid, dim3(kNT), 0, st, s); break;
+            default: hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_step<AUD_F16>), grid, dim3(kNT), 0, st, s);
+        }
+    });
 }
 
 }  // namespace aud

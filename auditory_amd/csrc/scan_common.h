@@ -65,7 +65,7 @@ struct Where {  // which channels, chunk and item a workgroup has
     int b, chunk, g, d0, dn, block;  // first channel, channels (<= 64), block within the group
     // (the first pass leaves the last chunk out, the gradients' first pass the first one)
     __device__ __forceinline__ Where(const ScanArgs& a, int blocks, int skip_last, int skip_first) {
-        int id = blockIdx.x;
+        int id = a.first + blockIdx.x;
         block = id % blocks;
         id /= blocks;
         g = id % a.G;
@@ -151,7 +151,7 @@ __device__ __forceinline__ void step_sizes(float (&dt)[E], int softp) {
 // past N and steps at and behind the item's length are 0.
 template <int DT>
 __global__ void __launch_bounds__(kNT) k_scan_table(ScanArgs a, int NP, int NW, int tiles) {
-    const int64_t i = int64_t(blockIdx.x) * kNT + threadIdx.x;
+    const int64_t i = int64_t(a.first + blockIdx.x) * kNT + threadIdx.x;
     const unsigned per = 2 * kT * NP, r = unsigned(i % per);
     const int n = int(r / (2 * kT * NW) * NW + r % NW), which = int(r / NW % 2);
     int64_t q = i / per;
@@ -210,7 +210,7 @@ __device__ __forceinline__ void chunk_state(const ScanArgs& a, const Where& at, 
 template <bool BACK>
 __global__ void __launch_bounds__(kJoinThreads) k_scan_join(ScanArgs a) {
     constexpr int kAhead = 16;
-    const int64_t id = int64_t(blockIdx.x) * kJoinThreads + threadIdx.x, per = int64_t(a.N) * a.Dn;
+    const int64_t id = int64_t(a.first + blockIdx.x) * kJoinThreads + threadIdx.x, per = int64_t(a.N) * a.Dn;
     if (id >= a.B * per) return;
     const int64_t b = id / per;
     const int n = int(id % per / a.Dn), d = int(id % a.Dn);
@@ -237,11 +237,20 @@ __global__ void __launch_bounds__(kJoinThreads) k_scan_join(ScanArgs a) {
     }
 }
 
+template <bool BACK>
+hipError_t run_join(const ScanArgs& a, hipStream_t st) {
+    return in_slices_of(a, (int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads, kJoinThreads, [&](dim3 grid, const ScanArgs& s) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<BACK>), grid, dim3(kJoinThreads), 0, st, s);
+    });
+}
+
 template <int DT>
-void run_table(const ScanArgs& a, int NP, int NW, hipStream_t st) {
+hipError_t run_table(const ScanArgs& a, int NP, int NW, hipStream_t st) {
     const int tiles = (a.L + kT - 1) / kT;
     const int64_t n = int64_t(a.B) * a.G * tiles * kT * 2 * NP;
-    if (n > 0) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_table<DT>), dim3(unsigned((n + kNT - 1) / kNT)), dim3(kNT), 0, st, a, NP, NW, tiles);
+    return in_slices_of(a, (n + kNT - 1) / kNT, kNT, [&](dim3 grid, const ScanArgs& s) {
+        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_table<DT>), grid, dim3(kNT), 0, st, s, NP, NW, tiles);
+    });
 }
 
 }  // namespace

@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_scan_grad(ScanArgs a, int blocks)
 // dB, dC: the blocks' partial sums added in order and rounded to the activations' type
 template <int DT>
 __global__ void __launch_bounds__(kNT) k_scan_bc(ScanArgs a, int blocks) {
-    const int64_t n = int64_t(a.B) * a.L * a.G * a.N, i = int64_t(blockIdx.x) * kNT + threadIdx.x;
+    const int64_t n = int64_t(a.B) * a.L * a.G * a.N, i = int64_t(a.first + blockIdx.x) * kNT + threadIdx.x;
     if (i >= 2 * n) return;
     const int64_t o = i < n ? i : i - n;
     const float* p = a.part_bc + (i < n ? 0 : blocks * n) + o;
@@ -426,22 +426,27 @@ __global__ void __launch_bounds__(kNT) k_scan_bc(ScanArgs a, int blocks) {
 template <int DT, int NW, int W, bool VEC>
 hipError_t run_grad(const ScanArgs& a, const ScanRoute& r, hipStream_t st) {
     constexpr int NP = W * NW;
-    const dim3 grid(unsigned(int64_t(a.B) * a.chunks * a.G * r.blocks));
+    const int64_t side = int64_t(a.B) * a.G * r.blocks;  // workgroups side by side in a chunk
     const size_t lds1 = size_t(2) * kT * kCh * 4, lds3 = size_t(3 * kT * kCh + 2 * kT * NP + 3 * W * kT * kCh) * 4;
     if (hipError_t e = allow_lds<&k_scan_grad<DT, NW, W, VEC, 3>>(lds3)) return e;
-    run_table<DT>(a, NP, NW, st);
+    if (hipError_t e = run_table<DT>(a, NP, NW, st)) return e;
     if (a.chunks > 1) {
-        const dim3 first(unsigned(int64_t(a.B) * (a.chunks - 1) * a.G * r.blocks));
-        hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, W, VEC, 1>), first, dim3(64 * W), lds1, st, a, r.blocks);
-        if (!a.fold) {
-            const unsigned join = unsigned((int64_t(a.B) * a.N * a.Dn + kJoinThreads - 1) / kJoinThreads);
-            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_join<true>), dim3(join), dim3(kJoinThreads), 0, st, a);
-        }
+        if (hipError_t e = in_slices_of(a, side * (a.chunks - 1), 64 * W, [&](dim3 grid, const ScanArgs& s) {
+                hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, W, VEC, 1>), grid, dim3(64 * W), lds1, st, s, r.blocks);
+            }))
+            return e;
+        if (!a.fold)
+            if (hipError_t e = run_join<true>(a, st)) return e;
     }
-    hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, W, VEC, 3>), grid, dim3(64 * W), lds3, st, a, r.blocks);
-    const int64_t bc = 2 * int64_t(a.B) * a.L * a.G * a.N;
-    if (bc > 0 && r.blocks > 1) hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_bc<DT>), dim3(unsigned((bc + kNT - 1) / kNT)), dim3(kNT), 0, st, a, r.blocks);
-    if (hipError_t e = hipGetLastError()) return e;
+    if (hipError_t e = in_slices_of(a, side * a.chunks, 64 * W, [&](dim3 grid, const ScanArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_grad<DT, NW, W, VEC, 3>), grid, dim3(64 * W), lds3, st, s, r.blocks);
+        }))
+        return e;
+    const int64_t bc = r.blocks > 1 ? 2 * int64_t(a.B) * a.L * a.G * a.N : 0;
+    if (hipError_t e = in_slices_of(a, (bc + kNT - 1) / kNT, kNT, [&](dim3 grid, const ScanArgs& s) {
+            hipLaunchKernelGGL(HIP_KERNEL_NAME(k_scan_bc<DT>), grid, dim3(kNT), 0, st, s, r.blocks);
+        }))
+        return e;
     return launch_column_sums(a.part, int64_t(a.B) * a.chunks, a.Dn, a.N, 2, a.dA, a.dD, a.ddelta_bias, st);
 }
 template <int DT, bool VEC>

@@ -21,6 +21,10 @@ FLAGS = {
     "fma": ["-O2", "-mfma", "-ffp-contract=fast"],
 }
 
+# threads a launch of the feature-map and frame-sequence operators may hold (2^32 - 1 on the GPU): small, so that grids go out in
+# slices here
+LAUNCH_THREADS = 4096
+
 
 def lib_path(variant="plain"):
     return os.path.join(HERE, "libauditory_emul%s.so" % ("" if variant == "plain" else "_" + variant))
@@ -44,7 +48,7 @@ def _build(variant, force):
     if not force and os.path.exists(out) and all(os.path.getmtime(d) <= os.path.getmtime(out) for d in deps):
         return out
     common = ["g++", "-std=c++17", "-fPIC", "-pthread"] + ([] if variant == "fma" else ["-ffp-contract=off"]) + [
-              "-Wall", "-Wno-unknown-pragmas", "-Wno-unused-function", "-Wno-attributes"] + FLAGS[variant] + [
+              "-DAUD_LAUNCH_THREADS=%d" % LAUNCH_THREADS, "-Wall", "-Wno-unknown-pragmas", "-Wno-unused-function", "-Wno-attributes"] + FLAGS[variant] + [
               "-I" + HERE, "-I" + product_build.INCLUDE, "-I" + product_build.CSRC]
     # one compile job per source, a few at a time (the sanitizer variants take a minute otherwise), then one link
     import tempfile

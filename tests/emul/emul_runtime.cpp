@@ -24,6 +24,7 @@
 thread_local dim3 threadIdx, blockIdx, blockDim, gridDim;
 extern "C" {
 int aud_emul_host_register_status = 0;
+long long aud_emul_launch_threads = 0xFFFFFFFFll;  // a launch of more threads is refused, as HIP refuses it
 }
 
 namespace aud {
@@ -118,6 +119,10 @@ void launch(dim3 grid, dim3 block, size_t lds_bytes, const std::function<void()>
     const int nthr = int(block.x * block.y * block.z);
     if (nthr < 1 || nthr > kMaxThreads || lds_bytes > sizeof(aud::aud_dyn_lds)) {
         g_last = hipErrorInvalidValue;
+        return;
+    }
+    if ((long long)grid.x * block.x > aud_emul_launch_threads) {
+        g_last = hipErrorInvalidConfiguration;
         return;
     }
     g_lds_bytes = lds_bytes;

@@ -1,10 +1,13 @@
-"""The feature-map and frame-sequence operators where a range ends: decays that pass float32 over a run of frames, launches past
-what one can hold, inputs that ask for gradients."""
+"""The feature-map and frame-sequence operators where a range ends: decays that pass float32 over a run of frames, inputs that ask
+for gradients, grids of more threads than a launch can hold."""
+import ctypes as C
+
 import pytest
 import torch
 
 import frame_cases as F
 import frame_ref as R
+import norm_cases as N
 from auditory_amd import capi, norm, scan
 from test_norm_widths import emu, emu_lib  # noqa: F401  (fixtures)
 
@@ -171,3 +174,96 @@ def test_emul_in_a_function(emu):  # noqa: F811
 @gpu
 def test_gpu_in_a_function():
     in_a_function("cuda:0")
+
+
+# ---- grids of more threads than a launch can hold ----------------------------------------------------------------------------
+
+@pytest.fixture
+def small_launches(emu):  # noqa: F811
+    """the emulator refuses launches past its build's limit"""
+    import build_emul
+    limit = C.c_longlong.in_dll(emu, "aud_emul_launch_threads")
+    before, limit.value = limit.value, build_emul.LAUNCH_THREADS
+    yield
+    limit.value = before
+
+
+SLICED = [
+    (N.case, (10, 3, 24, 3, "f32", "silu", True, None, 0)),                    # items held in registers, the gradients' item kernel
+    (N.case, (9, 6, 1300, 13, "bf16", "gelu", True, None, 0)),                 # items read twice, the parameters' column sums
+    (N.case, (5, 24, 1024, 1024, "f32", "none", True, None, 0)),               # chunks, many groups
+    (N.case, (2, 600, 32, 4, "f32", "silu", True, "mixed", 0)),                # chunks, joined by all
+    (F.conv_case, (5, 70, 130, 4, "bf16", "silu", True, True, "mixed", 1)),
+    (F.scan_case, (2, 34, 130, 2, 17, "f32", True, True, True, True, True, "mixed", 0)),   # two blocks a group, chunks
+    (F.scan_case, (33, 1, 65, 1, 4, "f32", True, True, True, True, True, None, 0)),        # one frame
+    (F.scan_case, (1, 560, 65, 1, 64, "f32", True, True, True, True, True, None, 0)),      # the gradients' chunks joined by a kernel
+]
+
+
+@pytest.mark.parametrize("i", range(len(SLICED)))
+def test_emul_launches_in_slices(small_launches, i):
+    fn, case = SLICED[i]
+    fn("cpu", *case)
+
+
+@gpu
+def test_gpu_norm_of_more_items_than_a_launch_holds():
+    """2^23 items and some of 512 threads each: every item as it comes out alone"""
+    dev, n, k = "cuda:0", 1 << 10, (1 << 13) + 1
+    m = F.Make(dev, 23, "bf16")
+    x, dy, w, b = m.n(n, 1, 16), m.n(n, 1, 16), m.n(16, f32=True), m.n(16, f32=True)
+    y, st = norm.group_norm(x, 4, w, b, act="silu", want_stats=True)
+    dx, dw, db = norm.group_norm_grad(dy, x, st, 4, w, b, act="silu")
+    many = lambda t: t.repeat(k, *[1] * (t.dim() - 1))  # noqa: E731
+    ys, sts = norm.group_norm(many(x), 4, w, b, act="silu", want_stats=True)
+    assert torch.equal(ys.view(k, n, 16), y.view(1, n, 16).expand(k, n, 16))
+    assert torch.equal(sts.view(k, n, 8), st.view(1, n, 8).expand(k, n, 8))
+    dxs, dws, dbs = norm.group_norm_grad(many(dy), many(x), sts, 4, w, b, act="silu")
+    assert torch.equal(dxs.view(k, n, 16), dx.view(1, n, 16).expand(k, n, 16))
+    # the sums over k n items: at most k n / 32 + 16 additions follow each other
+    e = N.Exact(x, dy, 4, w, b, 1e-5, "silu", None)
+    for got, one, bound in ((dws, dw, e.edw), (dbs, db, e.edb)):
+        terms = bound / R.U  # (the bound holds (S >= 1) u times the sum of the terms' absolute values)
+        assert ((got.cpu().double() - k * one.cpu().double()).abs() <= k * (bound + (k * n / 32 + 16) * R.U * terms)).all()
+
+
+@gpu
+def test_gpu_conv_of_more_threads_than_a_launch_holds():
+    """2^32 threads of one element, one frame each"""
+    dev, n = "cuda:0", 65537
+    m = F.Make(dev, 29, "bf16")
+    row, w, b = m.n(1, n), m.n(n, 1, f32=True), m.n(n, f32=True)
+    one = scan.causal_conv_step(row, None, w, b, act="silu")
+    x = row.expand(n, n).contiguous()
+    y = scan.causal_conv_step(x, None, w, b, act="silu")
+    assert all(torch.equal(y[i:i + 4096], one.expand(min(4096, n - i), n)) for i in range(0, n, 4096))
+
+
+@gpu
+def test_gpu_scans_of_more_threads_than_a_launch_holds():
+    dev = "cuda:0"
+    # one frame: 2^30 channels and some, four lanes each
+    items, ch = (1 << 15) + 1, 1 << 15
+    m = F.Make(dev, 31, "bf16")
+    u, delta, z = m.n(1, ch), m.n(1, ch), m.n(1, ch)
+    B, Cm, A = m.n(1, 1, 1), m.n(1, 1, 1), -m.u(ch, 1)
+    h = m.n(1, ch, 1, f32=True)
+    many = lambda t: t.expand(items, *t.shape[1:]).contiguous()  # noqa: E731
+    one = h.clone()
+    y = scan.selective_scan_step(u, delta, A, B, Cm, one, z=z, softplus=True)
+    state = many(h)
+    ys = scan.selective_scan_step(many(u), many(delta), A, many(B), many(Cm), state, z=many(z), softplus=True)
+    assert torch.equal(ys, many(y)) and torch.equal(state, many(one))
+    del ys, state
+    # 2^24 workgroups and some: a channel a group
+    items, ch = 17, 1 << 20
+    u, delta, dy = m.n(1, 2, ch), m.n(1, 2, ch), m.n(1, 2, ch)
+    B, Cm, A = m.n(1, 2, ch, 1), m.n(1, 2, ch, 1), -m.u(ch, 1)
+    y, kept = scan.selective_scan(u, delta, A, B, Cm, softplus=True, keep=True)
+    g = scan.selective_scan_grad(dy, u, delta, A, B, Cm, kept, softplus=True)
+    args = [many(u), many(delta), A, many(B), many(Cm)]
+    ys, kept = scan.selective_scan(*args, softplus=True, keep=True)
+    assert torch.equal(ys, many(y))
+    gs = scan.selective_scan_grad(many(dy), *args, kept, softplus=True)
+    for p, q in ((gs.u, g.u), (gs.delta, g.delta), (gs.B, g.B), (gs.C, g.C)):
+        assert torch.equal(p, many(q))
