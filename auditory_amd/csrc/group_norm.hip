@@ -33,7 +33,7 @@ struct Lanes {
     int cols, lanes, r, c;
     __device__ __forceinline__ Lanes(int n_packs, int first) {
         cols = n_packs - first < NT ? n_packs - first : NT;
-        lanes = SPREAD || n_packs <= NT ? NT / cols : 1;
+        lanes = NT / (SPREAD ? cols : n_packs < NT ? n_packs : NT);
         r = int(threadIdx.x) / cols;
         c = first + int(threadIdx.x) - r * cols;
         if (r >= lanes) r = 1 << 30;  // left over: no row is theirs

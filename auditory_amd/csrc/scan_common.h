@@ -54,12 +54,14 @@ __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2
 
 // 2^x h + part, x the exponent of a whole run of steps.  A run of growing steps can pass float32 where its product with a small h
 // does not, and h = 0 stays 0 whatever it is multiplied by: what x has above 120 goes into h first, by powers of two.  (500: more
-// than that takes the smallest h there is past float32.)
+// than that takes the smallest h there is past float32.)  The joins take the plain form, which ends in an infinity or NaN where this
+// one is wanted (neither goes away again), and only then this one: in every step it costs the join of 64 chunks 2 us of 6.
 __device__ __forceinline__ float carried(float x, float h, float part) {
     const float y = x > 500.f ? 500.f : x;
     const int n = y > 120.f ? int(ceilf(y - 120.f)) : 0;
     return fmaf(exp2_hw(y - float(n)), ldexpf(h, n), part);
 }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) <= 3.402823466e38f; }
 
 struct Where {  // which channels, chunk and item a workgroup has
     int b, chunk, g, d0, dn, block;  // first channel, channels (<= 64), block within the group
@@ -186,14 +188,14 @@ __device__ __forceinline__ void chunk_state(const ScanArgs& a, const Where& at, 
     }
     // forward: slots 1 .. chunk (slot 0 alone for chunk 0); back: slots chunks - 1 down to chunk + 1
     const int count = BACK ? a.chunks - 1 - at.chunk : (at.chunk > 0 ? at.chunk : 1);
+    auto slot_of = [&](int k) { return BACK ? a.chunks - 1 - k : (at.chunk > 0 ? 1 + k : 0); };
+    auto chunk_of = [&](int slot) { return BACK ? slot : (slot > 0 ? slot - 1 : 0); };
     for (int k = 0; k < count; k += kAhead) {
         float part[kAhead][NW], sum[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const int kk = k + j < count ? k + j : count - 1;
-            const int slot = BACK ? a.chunks - 1 - kk : (at.chunk > 0 ? 1 + kk : 0);
-            const int chunk = BACK ? slot : (slot > 0 ? slot - 1 : 0);
-            sum[j] = dt[int64_t(chunk) * a.Dn];
+            const int slot = slot_of(k + j < count ? k + j : count - 1);
+            sum[j] = dt[int64_t(chunk_of(slot)) * a.Dn];
 #pragma unroll
             for (int i = 0; i < NW; ++i) part[j][i] = n0 + i < a.N ? s[slot * per + int64_t(n0 + i) * a.Dn] : 0.f;
         }
@@ -201,7 +203,21 @@ __device__ __forceinline__ void chunk_state(const ScanArgs& a, const Where& at, 
         for (int j = 0; j < kAhead; ++j) {
             if (k + j >= count) break;
 #pragma unroll
-            for (int i = 0; i < NW; ++i) h[i] = k + j == 0 ? part[j][i] : carried(sum[j] * A2[i], h[i], part[j][i]);
+            for (int i = 0; i < NW; ++i) h[i] = k + j == 0 ? part[j][i] : fmaf(exp2_hw(sum[j] * A2[i]), h[i], part[j][i]);
+        }
+    }
+    bool plain = true;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) plain = plain && finite(h[i]);
+    if (!plain) {  // once more, slot by slot
+        for (int k = 0; k < count; ++k) {
+            const int slot = slot_of(k);
+            const float sum = dt[int64_t(chunk_of(slot)) * a.Dn];
+#pragma unroll
+            for (int i = 0; i < NW; ++i) {
+                const float part = n0 + i < a.N ? s[slot * per + int64_t(n0 + i) * a.Dn] : 0.f;
+                h[i] = k == 0 ? part : carried(sum * A2[i], h[i], part);
+            }
         }
     }
 }
@@ -221,19 +237,26 @@ __global__ void __launch_bounds__(kJoinThreads) k_scan_join(ScanArgs a) {
     float h = 0.f;
     for (int k = 0; k < a.chunks - 1; k += kAhead) {
         float mine[kAhead], sum[kAhead];
+        const float before = h;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int kk = k + j < a.chunks - 1 ? k + j : a.chunks - 2, slot = BACK ? a.chunks - 1 - kk : 1 + kk;
             mine[j] = s[slot * per];
             sum[j] = dt[int64_t(BACK ? slot : slot - 1) * a.Dn];
         }
+        auto walk = [&](auto join) {
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            if (k + j >= a.chunks - 1) break;
-            const int slot = BACK ? a.chunks - 1 - (k + j) : 1 + k + j;
-            h = k + j == 0 ? mine[j] : carried(sum[j] * A2, h, mine[j]);
-            s[slot * per] = h;
-        }
+            for (int j = 0; j < kAhead; ++j) {
+                if (k + j >= a.chunks - 1) break;
+                const int slot = BACK ? a.chunks - 1 - (k + j) : 1 + k + j;
+                h = k + j == 0 ? mine[j] : join(sum[j] * A2, h, mine[j]);
+                s[slot * per] = h;
+            }
+        };
+        walk([](float x, float v, float part) { return fmaf(exp2_hw(x), v, part); });
+        if (finite(h)) continue;
+        h = before;
+        walk([](float x, float v, float part) { return carried(x, v, part); });
     }
 }
 
