@@ -64,6 +64,12 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
         if (there && at.chunk == 0 && PASS == 1) a.sums[(int64_t(at.b) * a.chunks * a.N + n) * a.Dn + d] = h[i];
     }
     if (PASS == 3 && a.chunks > 1) chunk_state<NW, false>(a, at, wave * NW, d, live, A2, h);
+    if (tiles == 0) {  // no frame at all: the buffers may be null, so nothing below points into them
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+            if (PASS == 3 && live && wave * NW + i < a.N && a.state_out) a.state_out[(int64_t(at.b) * a.Dn + d) * a.N + wave * NW + i] = h[i];
+        return;
+    }
     float skip[E], bias[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -76,11 +82,10 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
     // addresses of this thread's channels in its row of the tile, moved on by 16 rows a tile (rows behind the last one: the last)
     typedef typename Elem<DT>::raw raw;
     const int cc = c < at.dn ? c : 0, left = at.dn - cc;
-    const bool any = first < end;  // (no frame at all: the buffers may be null, nothing is pointed at)
     const int64_t row = first * kT + pt;
-    const raw* pu = any ? static_cast<const raw*>(a.u) + u0 + row * a.ur + cc : nullptr;
-    const raw* pd = any ? static_cast<const raw*>(a.delta) + e0 + row * a.er + cc : nullptr;
-    const raw* pz = a.z && any ? static_cast<const raw*>(a.z) + z0 + row * a.zr + cc : pu;  // (no gate: read and not used)
+    const raw* pu = static_cast<const raw*>(a.u) + u0 + row * a.ur + cc;
+    const raw* pd = static_cast<const raw*>(a.delta) + e0 + row * a.er + cc;
+    const raw* pz = a.z ? static_cast<const raw*>(a.z) + z0 + row * a.zr + cc : pu;  // (no gate: read and not used)
     const int64_t su = kT * a.ur, sd = kT * a.er, sz = a.z ? kT * a.zr : su;
     auto fetch = [&](int tile) {
         if ((tile + 1) * kT > a.L) {  // (the last tile: the addresses are not moved on from here)
@@ -91,8 +96,8 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
         rd.load(pd, left);
         if (PASS == 3) rz.load(pz, left);
     };
-    float* pk = a.kept && any ? a.kept + ((int64_t(at.b) * tiles + first) * a.N + wave * NW) * a.Dn + d : nullptr;
-    raw* py = PASS == 3 && any ? static_cast<raw*>(a.y) + y0 + int64_t(first * kT + pt) * a.Dn : nullptr;
+    float* pk = a.kept ? a.kept + ((int64_t(at.b) * tiles + first) * a.N + wave * NW) * a.Dn + d : nullptr;
+    raw* py = PASS == 3 ? static_cast<raw*>(a.y) + y0 + int64_t(first * kT + pt) * a.Dn : nullptr;
     float u[2][E], z[2][E];  // of the tile that is being scanned, and of the next one
     auto stage = [&](int tile, int buf) {
         float step[2 * E], dt[E];
@@ -112,17 +117,17 @@ __global__ void __launch_bounds__(64 * W) k_scan(ScanArgs a, int blocks) {
         }
         lds_write(lds + 2 * ((buf * kT + pt) * kCh + c), step);
     };
-    if (any) {
+    if (first < end) {
         fetch(first);
         stage(first, 0);
     }
     __syncthreads();
-    ScalarTable bc = (ScalarTable)(any ? a.table + ((int64_t(at.b) * a.G + at.g) * tiles + first) * kT * 2 * NP + wave * kT * 2 * NW : nullptr);
+    ScalarTable bc = (ScalarTable)(a.table + ((int64_t(at.b) * a.G + at.g) * tiles + first) * kT * 2 * NP + wave * kT * 2 * NW);
     typedef Vectors<NW> Vec;
     constexpr int GS = Vec::GS;
     Vec next{};
     wait_loads();
-    if (any) next.template load<true, PASS == 3>(bc);
+    if (first < end) next.template load<true, PASS == 3>(bc);
     auto scan_tile = [&](int tile, auto which) {  // (a turn of the loop for each buffer: what belongs to one stays in its registers)
         constexpr int buf = decltype(which)::value;
         const bool more = tile + 1 < end;
