@@ -31,6 +31,9 @@ def stale():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
+NO_PACKED = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def _flags():
     # -fno-slp-vectorize: hipcc otherwise packs neighbouring f32 adds/muls of the butterflies into
     # v_pk_* instructions, which on gfx950 issue no faster than two scalar ops (measured: profiles/
@@ -38,8 +41,8 @@ def _flags():
     # -packed-fp32-ops: no packed float32 instructions at all (hipcc makes them from ordinary float code too): some of their forms
     # have given wrong results on this hardware now and then, without an error (the host pass warns that it does not know the feature)
     # -amdgpu-kernarg-preload-count: leading scalar kernel arguments arrive in SGPRs with the wave (wave_common.h wave_kernel_t)
-    return ["--offload-arch=gfx950", "-O3", "-fno-slp-vectorize", "-std=c++17", "-fPIC", "-mllvm", "-amdgpu-kernarg-preload-count=" + os.environ.get("AUD_KERNARG_PRELOAD", "16"),
-            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-Xarch_host", "-ffp-contract=off", "-I" + INCLUDE, "-I" + CSRC]
+    return ["--offload-arch=gfx950", "-O3", "-fno-slp-vectorize", "-std=c++17", "-fPIC", "-mllvm", "-amdgpu-kernarg-preload-count=" + os.environ.get("AUD_KERNARG_PRELOAD", "16")] + \
+        NO_PACKED + ["-Xarch_host", "-ffp-contract=off", "-I" + INCLUDE, "-I" + CSRC]
 
 
 def build(force=False, verbose=False, stamps=False, tag=None, defines=()):
@@ -110,7 +113,7 @@ def build_stream_read(force=False):
     """tools/ubench/libstream_read.so: the plain float32 read kernel bench.py times for `roofline.measured_read_GBps` (SURVEY 8d's
     measured HBM-read roof).  Measurement only: the product library neither contains nor loads it."""
     if force or not os.path.exists(UBENCH_LIB) or os.path.getmtime(UBENCH_LIB) < os.path.getmtime(UBENCH_SRC):
-        subprocess.check_call([_hipcc(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-o", UBENCH_LIB, UBENCH_SRC])
+        subprocess.check_call([_hipcc(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED + ["-shared", "-o", UBENCH_LIB, UBENCH_SRC])
     return UBENCH_LIB
 
 

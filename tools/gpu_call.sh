@@ -45,17 +45,17 @@ for step in "$@"; do
                     python3 "$OLDPWD/bench.py" --only-headline --no-cpu-baseline --min-seconds 0.05 > "$OLDPWD/gpurun_out/${TAG}_trace.log" 2>&1)
                rc=$?; echo "[gpu_call] trace rc=$rc"; if [ $rc -eq 124 ] || [ $rc -ge 128 ]; then exit $rc; fi
                python3 tools/trace_overlap.py "gpurun_out/trace_${TAG}" > "gpurun_out/${TAG}_graph_overlap.txt" 2>&1; cat "gpurun_out/${TAG}_graph_overlap.txt" ;;
-        ubench) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O2 -o /tmp/valu_rates valu_rates.hip) &&
+        ubench) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o /tmp/valu_rates valu_rates.hip) &&
                 run ubench 120 /tmp/valu_rates ;;
-        mfma) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O2 -o /tmp/mfma_beside_valu mfma_beside_valu.hip) &&
+        mfma) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o /tmp/mfma_beside_valu mfma_beside_valu.hip) &&
                 run mfma 120 /tmp/mfma_beside_valu ;;
-        stream) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O2 -DSTREAM_READ_MAIN -o /tmp/stream_read stream_read.hip) &&
+        stream) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -DSTREAM_READ_MAIN -o /tmp/stream_read stream_read.hip) &&
                 run stream 120 /tmp/stream_read ;;
         runlib:*) args=$(echo "${step#runlib:}" | tr ',' ' ')   # runlib:TAG,script.py,args...  (an experimental build, tools/run_with_lib.py)
                run runlib$i 400 python tools/run_with_lib.py $args
                grep '^{' "gpurun_out/${TAG}_runlib$i.log" | tail -1 > "gpurun_out/${TAG}_runlib$i.json" ;;
         tune_bluestein) run tune_bluestein 1000 bash tools/tune_bluestein.sh ;;
-        wstream) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O2 -o /tmp/stream_write stream_write.hip) &&
+        wstream) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o /tmp/stream_write stream_write.hip) &&
                 run wstream 120 /tmp/stream_write ;;
         two_ranks) run two_ranks 500 bash tools/two_ranks_one_gpu.sh "${TAG}_two" ;;
         ranks:*) run ranks${step#ranks:} 500 bash tools/two_ranks_one_gpu.sh "${TAG}_ranks${step#ranks:}" "${step#ranks:}" ;;
@@ -64,7 +64,7 @@ for step in "$@"; do
         sweep) run sweep 600 python tools/rate_sweep.py --json "gpurun_out/${TAG}_rate_sweep.json" ;;
         sweep:*) args=$(echo "${step#sweep:}" | tr ',' ' ')
                run sweep$i 600 python tools/rate_sweep.py --json "gpurun_out/${TAG}_rate_sweep$i.json" $args ;;
-        dispatch) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -O2 -o /tmp/dispatch_rate dispatch_rate.hip) &&
+        dispatch) (cd tools/ubench && /opt/rocm/bin/hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O2 -o /tmp/dispatch_rate dispatch_rate.hip) &&
                 run dispatch 120 /tmp/dispatch_rate ;;
         *) echo "unknown step $step"; exit 2 ;;
     esac

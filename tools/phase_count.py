@@ -30,7 +30,7 @@ def main():
     src = "melspec_%s.hip" % next(w for w in ("w16", "w20", "w64") if w in key)
     with tempfile.TemporaryDirectory() as tmp:
         out = os.path.join(tmp, "wave.s")
-        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fno-slp-vectorize", "-std=c++17",
+        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-fno-slp-vectorize", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                                "-DAUD_PHASE_MARKERS", "-I" + os.path.join(ROOT, "include"),
                                "-I" + os.path.join(ROOT, "auditory_amd", "csrc"), "-x", "hip", "--cuda-device-only", "-S",
                                os.path.join(ROOT, "auditory_amd", "csrc", src), "-o", out],
