@@ -6,7 +6,7 @@
 //
 // Statistics: a thread sums x - k and (x - k)^2 of its rows of a channel, k the first of them, and turns the pair into a mean
 // and a sum of squared distances from it; those are joined (rows, channels, chunks of rows) by
-//   M2 = sum M2_i + n_i (m_i - m)^2, which has no cancellation, so a level far from zero costs nothing.
+//   M2 = sum M2_i + n_i (m_i - m)^2, which has no cancellation, so a level far from zero costs no more than the mean's own rounding.
 // Rows at and behind lengths[b] are not read; their results are zero.
 //
 // Three routes by the size of an item.  Up to four packs a thread it stays in one workgroup's registers: read once, one launch
@@ -15,8 +15,8 @@
 // then every workgroup joins its item's and writes (gradients: channel sums, joined per item, then dx, the parameters' sums by
 // workgroups of their own behind them).  Memory bounds that route: 16 x 4096 x 512 bfloat16 forward 15 + 28 us (67 MB read, then 134
 // moved), gradients 28 + 5 + 36 us (134, then 201 MB), 109 us a pass on inputs that the Infinity Cache holds, 123 on others, where
-// one sweep of everything would be 65; an item of 4 MB is more than a CU holds, and workgroups that wait for one another inside a
-// launch are not used here.
+// one sweep of everything would be 65.  An item is the unit here, and its 4 MB are more than a CU holds; the statistics need only a
+// group of it, 128 KB there, which one or two workgroups' registers would hold.  A route by (item, group) is not built.
 #include "frame_ops.h"
 
 namespace aud {

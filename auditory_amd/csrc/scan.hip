@@ -23,11 +23,14 @@
 // The vector pipe bounds it, not memory: a state and step is one exponential (8 cycles of a SIMD) and four products and fused
 // products (4 cycles each), a channel and step about 50 more instructions (softplus, gate, conversions, the sum over the waves).
 // 8 x 2048 x 1536, 16 states, bfloat16: 178 us, 204 MB (floor 40 us); 192 workgroups, one a CU, whose SIMDs issue vector
-// instructions 75 % of the time.  Gradients, 4 x 2048 x 1024: 41 us the first scan, 126 the second (82 %), of 255 for values and
-// gradients.  What was measured on the way there: B and C broadcast from LDS 243 us; scalar loads without a group in hand 638, as
-// runs of 64 bytes a group ahead 207; one barrier a tile instead of two 190; both elements of a thread side by side 186; addresses
-// moved on by a tile, a turn of the loop for each LDS buffer 178.  Not taken: the steps' LDS reads a group ahead 182, the output of
-// a tile behind the next one's scan 192, groups of half the size 194; inputs that lie still in the caches change nothing.
+// instructions 75 % of the time.  Gradients, 4 x 2048 x 1024: 40 us the first scan, 122 the second (82 %), of 255 for values and
+// gradients.  The first scans of a cut axis, 40 us each of values and of gradients there, issue 60 % of the time only; what they wait
+// for in the rest (a barrier every 16 steps with little between, 448 workgroups on 256 CUs) was not taken apart.
+//
+// What was measured on the way to 178: B and C broadcast from LDS 243 us; scalar loads without a group in hand 638, as runs of 64
+// bytes a group ahead 207; one barrier a tile instead of two 190; both elements of a thread side by side 186; addresses moved on by a
+// tile, a turn of the loop for each LDS buffer 178.  Not taken: the steps' LDS reads a group ahead 182, the output of a tile behind
+// the next one's scan 192, groups of half the size 194; inputs that lie still in the caches change nothing.
 #include <type_traits>
 
 #include "scan_common.h"

@@ -569,7 +569,8 @@ int aud_scan_batch_dev(aud_ctx* ctx, const aud_scan_params* p, const void* u, co
                        int64_t workspace_bytes, void* stream);
 /* kept: as aud_scan_batch_dev wrote it for the same inputs.  dstate_out: gradient of state_out, or NULL.  du, ddelta (and dz
  * where z is given) [n_items, steps, channels]; dB, dC [n_items, steps, groups, states]; dA float32 [channels, states]; dD,
- * ddelta_bias float32 [channels], dstate float32 [n_items, channels, states]: or NULL. */
+ * ddelta_bias float32 [channels], dstate float32 [n_items, channels, states]: or NULL.  Where a frame that counts holds an
+ * infinite B or C, dB and dC may be NaN in place of an infinity. */
 int aud_scan_grad_dev(aud_ctx* ctx, const aud_scan_params* p, const void* dy, const void* u, const void* delta, const float* A,
                       const void* B, const void* C, const float* D, const void* z, const float* delta_bias,
                       const int32_t* lengths, const float* kept, const float* dstate_out, void* du, void* ddelta, float* dA,

@@ -23,7 +23,7 @@ FLAGS = {
 
 # threads a launch of the feature-map and frame-sequence operators may hold (2^32 - 1 on the GPU): small, so that grids go out in
 # slices here
-LAUNCH_THREADS = 4096
+LAUNCH_THREADS = 2048
 
 
 def lib_path(variant="plain"):

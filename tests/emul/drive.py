@@ -26,8 +26,8 @@ def frames_cases(lib, variant):
     native = frames.native()
     frames.context = lambda x, name: runtime.get_ctx(0).handle.value
     frames.bind(native, lib, False)
-    wide = [c for c in N.WIDE if c[:3] in ((2, 6, 257), (2, 40, 257), (2, 40, 301), (2, 6, 513), (1, 3, 2052), (1, 7, 2056), (2, 9, 1540))]
-    runs = [(N.case, c) for c in wide + N.ROUTES[:3]] + [(F.norm_case, c) for c in F.NORM[:4]]
+    few = ((2, 6, 257, "f16"), (2, 40, 257, "f32"), (2, 40, 301, "f32"), (2, 6, 513, "f32"), (1, 3, 2052, "f32"), (1, 7, 2056, "bf16"), (2, 9, 1540, "bf16"))
+    runs = [(N.case, c) for c in N.WIDE + N.ROUTES[2:3] if c[:3] + c[4:5] in few or c in N.ROUTES] + [(F.norm_case, c) for c in F.NORM[:4]]
     runs += [(F.conv_case, c) for c in F.CONV] + [(F.scan_case, c) for c in F.SCAN]
     if variant == "tsan":
         runs = [(N.case, (1, 3, 24, 3, "f32", "silu", True, None, 0)), (N.case, (1, 130, 65, 5, "f32", "silu", True, None, 0)),

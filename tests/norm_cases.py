@@ -173,8 +173,8 @@ WIDE += [
     (1, 2, 4095, 5, "f32", "silu", True, None, 0),
     (2, 3, 4096, 64, "f32", "silu", False, None, 0),
 ]
-# (on the emulator: every width in one workgroup, and over several in float32 and one of the others)
-WIDE_EMUL = [c for i, c in enumerate(WIDE) if not (c[1] in (40, 70) and c[4] == ("bf16", "f16")[list(WIDTHS).index(c[2]) % 2])]
+# (on the emulator: every width on both sides, in one of the types)
+WIDE_EMUL = [c for c in WIDE if c[2] not in WIDTHS or c[4] == ("f32", "bf16", "f16")[list(WIDTHS).index(c[2]) % 3]]
 # the other widths, every route: values held in registers, an item read twice, chunks joined by all or by a kernel of their own
 ROUTES = [
     (3, 7, 40, 8, "f32", "silu", True, "mixed", 0),

@@ -196,7 +196,7 @@ SLICED = [
     (F.conv_case, (5, 70, 130, 4, "bf16", "silu", True, True, "mixed", 1)),
     (F.scan_case, (2, 34, 130, 2, 17, "f32", True, True, True, True, True, "mixed", 0)),   # two blocks a group, chunks
     (F.scan_case, (33, 1, 65, 1, 4, "f32", True, True, True, True, True, None, 0)),        # one frame
-    (F.scan_case, (1, 560, 65, 1, 64, "f32", True, True, True, True, True, None, 0)),      # the gradients' chunks joined by a kernel
+    (F.scan_case, (1, 560, 65, 1, 32, "f32", True, True, True, True, True, None, 0)),      # the gradients' chunks joined by a kernel
 ]
 
 

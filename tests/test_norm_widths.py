@@ -61,7 +61,7 @@ def test_gpu_routes(case):
 
 # ---- that the bounds see what they are there to see -----------------------------------------------------------------------
 
-SEEN = [N.ROUTES[0], N.ROUTES[2], N.ROUTES[3], N.ROUTES[5], N.ROUTES[6], (2, 40, 301, 7, "f32", "silu", True, None, 0)]
+SEEN = [N.ROUTES[0], N.ROUTES[2], N.ROUTES[3], N.ROUTES[5], N.ROUTES[7], (2, 40, 301, 7, "f32", "silu", True, None, 0)]
 
 
 @pytest.mark.parametrize("case", SEEN, ids=ids(SEEN))
