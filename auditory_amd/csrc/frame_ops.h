@@ -9,6 +9,13 @@
 
 namespace aud {
 
+// an index into a table of LDS: the CPU thread emulator's build ends the process where it is outside
+#if defined(__clang__)
+#define AUD_IN_TABLE(at, size) ((void)0)
+#else
+#define AUD_IN_TABLE(at, size) ((at) >= 0 && (at) < (size) ? (void)0 : std::abort())
+#endif
+
 // ---- element types: `raw` as stored, up() exact to float32, down() rounds to nearest even ------------------------------
 template <int DT>
 struct Elem;

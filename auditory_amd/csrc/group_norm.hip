@@ -130,6 +130,7 @@ __device__ __forceinline__ void group_moments(const NormArgs& a, int b, int lo, 
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 const int at = l.r * width + l.c * V + i;
+                AUD_IN_TABLE(at, size);
                 e_mean[at] = fmaf(s[i], inv, k[i]);
                 e_m2[at] = fmaxf(ss[i] - s[i] * s[i] * inv, 0.f) + 0.f * ss[i];  // (NaN stays NaN)
             }
@@ -269,7 +270,10 @@ __global__ void __launch_bounds__(kItemThreads) k_norm_held(NormArgs a) {
                 for (int i = 0; i < V; ++i) part[i] += __shfl_xor(part[i], s);
         if (mine && (!fold || int(threadIdx.x & 63) < l.cols)) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) entries[run * a.C + l.c * V + i] = part[i];
+            for (int i = 0; i < V; ++i) {
+                AUD_IN_TABLE(run * a.C + l.c * V + i, NT / packs * a.C);
+                entries[run * a.C + l.c * V + i] = part[i];
+            }
         }
         __syncthreads();
         for_groups<NT>(a.G, [&](int g, int lane, int q, bool there) {
@@ -419,6 +423,7 @@ __device__ __forceinline__ void channel_sums(const NormArgs& a, int b, int lo, i
                      });
 #pragma unroll
         for (int i = 0; i < V; ++i) {
+            AUD_IN_TABLE(l.r * a.C + l.c * V + i, size);
             entries[l.r * a.C + l.c * V + i] = s0[i];
             entries[size + l.r * a.C + l.c * V + i] = s1[i];
         }

@@ -71,3 +71,25 @@ def test_lengths_are_checked(emu):  # noqa: F811
     huge = torch.tensor([2 ** 31 - 1, -2 ** 31], dtype=torch.int32)   # held to [0, frames]
     y = bp.group_norm(torch.ones(2, 3, 4, 8), 2, bias=torch.ones(8), lengths=huge)
     assert (y[0] == 1).all() and (y[1] == 0).all()
+
+
+@gpu
+def test_gpu_padded_maps_in_a_graph():
+    """captured once, replayed with other maps and lengths in the same buffers, eager work in between"""
+    dev = "cuda:0"
+    m = F.Make(dev, 19, "f32")
+    bp = BatchProcessor.__new__(BatchProcessor)
+    maps, w, b = m.n(4, 5, 9, 2, 4), m.n(8, f32=True), m.n(8, f32=True)
+    lengths = torch.tensor([9, 3, 0, 7], dtype=torch.int32, device=dev)
+    bp.group_norm(maps, 2, w, b, act="silu", lengths=lengths)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = bp.group_norm(maps, 2, w, b, act="silu", lengths=lengths)
+    for turn in range(4):
+        maps.copy_(m.n(4, 5, 9, 2, 4))
+        lengths.copy_(torch.tensor([turn, 9, 5 - turn, 20], dtype=torch.int32))
+        g.replay()
+        want = bp.group_norm(maps, 2, w, b, act="silu", lengths=lengths)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), turn
